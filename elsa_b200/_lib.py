@@ -9,7 +9,7 @@ from __future__ import annotations
 import ctypes
 import os
 import warnings
-from ctypes import c_char_p, c_int, c_int64, c_uint, c_uint64, c_void_p, POINTER
+from ctypes import c_char_p, c_double, c_int, c_int64, c_uint, c_uint64, c_void_p, POINTER
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 # ELSA_B200_LIB points the loader at another build of the same library (a tuning build, an installed copy)
@@ -62,6 +62,7 @@ SIGNATURES = {
     "elsa_twopass_backward": (c_int, [_P] * 7 + _BIAS + [_P, _P, _P] + _BIAS + [_P, c_int64] + [c_int] * 6 + [c_uint, _P]),
     "elsa_backward_shard_workspace_bytes": (c_int64, [c_int] * 5 + [c_uint]),
     "elsa_twopass_backward_shard": (c_int, [_P] * 11 + [c_int64] + [c_int] * 8 + [c_uint, _P]),
+    "elsa_rotary": (c_int, [_P, _P, _P, c_int, _P, _P, _P, c_int, _P, _P, c_int, c_int64, c_int64, c_double] + [c_int] * 7 + [_P]),
 }
 
 _lib = None

@@ -125,6 +125,11 @@ int bwd_simt(const BwdParams& p, int dtype, cudaStream_t st);
 // q' = fp16(q * fp16(c)), the product formed in fp16 (phase2.cu)
 int prescale_q_f16(const void* q, void* q_scaled, int64_t n_elems, float c, cudaStream_t st);
 
+// rotary positions (rotary.cu)
+int rotary(const void* q, void* q_out, const int64_t* qs, int q_heads, const void* k, void* k_out, const int64_t* ks, int k_heads,
+           const double* frequencies, const void* positions, int position_bytes, int64_t psb, int64_t psn, double magnitude,
+           int dtype, int batch, int n, int head_dim, int rotary_dim, int interleaved, int inverse, cudaStream_t st);
+
 // phase 2 (phase2.cu)
 // out_strides == nullptr: out is [bh, n_ctx, head_dim] contiguous; else `heads` splits bh and out is addressed by strides
 int merge_final_any(const float* m, const float* z, const void* s, void* out, float* row_m, float* row_z,

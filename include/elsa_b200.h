@@ -339,6 +339,22 @@ int elsa_twopass_backward_shard(const void* q, const void* k_shard, const void* 
                                 int dtype, int batch, int heads, int n_ctx, int head_dim, int n_keys,
                                 int key_offset, int is_causal, unsigned flags, void* stream);
 
+/* ---- operators of decoder models (no counterpart in the reference) -------------------------------------------------- */
+
+/* Rotary positions: the first rotary_dim dimensions of every row of q and k, as points of the plane -- dimensions (i, i + R/2),
+ * or neighbours (2i, 2i+1) where `interleaved` -- are turned by position * frequencies[i] and multiplied by `magnitude`; the
+ * other dimensions are copied.  `inverse` turns back (the gradient of the map).
+ * q, q_out: [batch, q_heads, n, head_dim] views, `q_strides` = {batch, head, row} element strides of q, then of q_out; k, k_out
+ * alike with k_heads heads, or k NULL (then k_out, k_strides and k_heads are not looked at).  The elements of a row are
+ * contiguous; any other stride and alignment will do, 16-byte aligned rows are faster.  Output == input with equal strides
+ * works in place.
+ * frequencies: rotary_dim / 2 doubles on the device.  positions: 64-bit (position_bytes 8) or 32-bit (4) signed integers at
+ * positions[b * position_stride_b + r * position_stride_n]; NULL with position_bytes 0: row r has position r. */
+int elsa_rotary(const void* q, void* q_out, const int64_t* q_strides, int q_heads, const void* k, void* k_out,
+                const int64_t* k_strides, int k_heads, const double* frequencies, const void* positions, int position_bytes,
+                int64_t position_stride_b, int64_t position_stride_n, double magnitude, int dtype, int batch, int n,
+                int head_dim, int rotary_dim, int interleaved, int inverse, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,87 @@
+"""CPU checks of the decoder-side operators: what they refuse, in Python and at the C ABI, and the host-side formulas."""
+import math
+
+import pytest
+import torch
+
+import elsa_b200 as E
+
+
+@pytest.fixture(scope="module")
+def lib():
+    from elsa_b200 import _lib, build
+    build.build()
+    return _lib.load()
+
+
+# ---- rotary -----------------------------------------------------------------------------------------------------
+def test_rotary_frequencies_plain_and_scaled():
+    plain, one = E.rotary_frequencies(8, base=10000.0)
+    assert plain.dtype == torch.float64 and one == 1.0
+    assert plain.tolist() == pytest.approx([1.0, 0.1, 0.01, 0.001], rel=1e-14)
+    linear, _ = E.rotary_frequencies(8, scaling="linear", factor=4.0)
+    assert torch.allclose(linear, plain / 4, rtol=1e-15)
+    ntk, _ = E.rotary_frequencies(8, scaling="ntk", factor=4.0)
+    assert ntk[0] == 1.0 and float(ntk[-1]) == pytest.approx(float(plain[-1]) / 4, rel=1e-12)
+
+
+def test_rotary_yarn_keeps_fast_pairs_and_divides_slow_ones():
+    r, original, factor = 128, 4096, 16.0
+    plain, _ = E.rotary_frequencies(r)
+    yarn, magnitude = E.rotary_frequencies(r, scaling="yarn", factor=factor, original_positions=original)
+    assert magnitude == pytest.approx(0.1 * math.log(factor) + 1.0)
+    turns = plain * original / (2 * math.pi)
+    index = torch.arange(r // 2)
+    fast, slow = index[turns > 32.0][:-1], index[turns < 1.0][1:]     # (the borders round outward by at most one pair)
+    assert len(fast) > 5 and len(slow) > 5
+    assert torch.equal(yarn[fast], plain[fast])
+    assert torch.allclose(yarn[slow], plain[slow] / factor, rtol=1e-14)
+    ratio = (yarn / plain)
+    assert bool((ratio[1:] <= ratio[:-1] + 1e-15).all()) and float(ratio.min()) >= 1 / factor - 1e-15
+
+
+@pytest.mark.parametrize("kwargs,match", [
+    (dict(rotary_dim=7), "rotary_dim"), (dict(rotary_dim=0), "rotary_dim"), (dict(rotary_dim=258), "rotary_dim"),
+    (dict(rotary_dim=8, base=0.0), "base"), (dict(rotary_dim=8, base=math.inf), "base"),
+    (dict(rotary_dim=8, scaling="cubic"), "scaling"), (dict(rotary_dim=8, scaling="linear", factor=0.5), "factor"),
+    (dict(rotary_dim=2, scaling="ntk", factor=2.0), "rotary_dim"), (dict(rotary_dim=8, scaling="yarn", factor=2.0), "original"),
+    (dict(rotary_dim=8, scaling="yarn", factor=2.0, original_positions=64, beta_fast=1.0, beta_slow=2.0), "beta_fast"),
+])
+def test_rotary_frequencies_refusals(kwargs, match):
+    with pytest.raises(ValueError, match=match):
+        E.rotary_frequencies(**kwargs)
+
+
+def test_rotary_embedding_refuses_cpu_tensors_and_wrong_shapes():
+    q, f = torch.randn(1, 2, 8, 4), torch.ones(2, dtype=torch.float64)
+    with pytest.raises(ValueError, match="CUDA"):
+        E.rotary_embedding(q, None, f)
+    with pytest.raises(ValueError, match="shape"):
+        E.rotary_embedding(q[0], None, f)
+    with pytest.raises(ValueError, match="agree"):
+        E.rotary_embedding(q, q[:, :, :4], f)
+
+
+def test_rotary_overlap_check():
+    from elsa_b200.rotary import _overlaps
+    base = torch.zeros(2, 3, 5, 8)
+    assert not _overlaps(base) and not _overlaps(base.transpose(1, 2)) and not _overlaps(base[:, :, ::2])
+    assert _overlaps(base[:1].expand(4, 3, 5, 8)) and _overlaps(base.as_strided((2, 3, 5, 8), (120, 40, 4, 1)))
+    assert not _overlaps(base[:1, :1, :1])
+
+
+def test_rotary_abi_refuses_before_any_launch(lib):
+    import ctypes
+    st = (ctypes.c_int64 * 6)(512, 256, 64, 512, 256, 64)
+    other = (ctypes.c_int64 * 6)(512, 256, 64, 512, 64, 256)
+
+    def call(q=64, q_out=128, strides=st, heads=2, k=None, k_out=None, ks=None, kh=0, freq=64, pos=None, pos_bytes=0, dtype=1, batch=1,
+             n=4, d=64, r=64):
+        return lib.elsa_rotary(q, q_out, strides, heads, k, k_out, ks, kh, freq, pos, pos_bytes, 0, 1, 1.0, dtype, batch, n, d, r, 0, 0, None)
+
+    assert call(q=None) == 1 and call(q_out=None) == 1 and call(strides=None) == 1 and call(freq=None) == 1
+    assert call(heads=0) == 1 and call(n=0) == 1 and call(batch=0) == 1 and call(dtype=9) == 1
+    assert call(k=64) == 1 and call(k=64, k_out=64, ks=st, kh=0) == 1
+    assert call(r=65) == 2 and call(r=0) == 2 and call(d=64, r=128) == 2 and call(d=2048) == 2 and call(d=512, r=512) == 2
+    assert call(pos=64, pos_bytes=0) == 1 and call(pos=None, pos_bytes=8) == 1 and call(pos=64, pos_bytes=2) == 1
+    assert call(q=64, q_out=64, strides=other) == 1
