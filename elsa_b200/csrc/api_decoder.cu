@@ -26,7 +26,7 @@ extern "C" int elsa_rotary(const void* q, void* q_out, const int64_t* q_strides,
   // in place means the same elements: a row written where another one is still to be read would be lost
   if (q == q_out && !std::equal(q_strides, q_strides + 3, q_strides + 3)) return ELSA_ERR_INVALID_ARGUMENT;
   if (k && k == k_out && !std::equal(k_strides, k_strides + 3, k_strides + 3)) return ELSA_ERR_INVALID_ARGUMENT;
-  if (static_cast<int64_t>(q_heads) + (k ? k_heads : 0) > 65536) return ELSA_ERR_UNSUPPORTED;
+  if (static_cast<int64_t>(q_heads) + (k ? k_heads : 0) > 2048) return ELSA_ERR_UNSUPPORTED;
   return rotary(q, q_out, q_strides, q_heads, k, k_out, k_strides, k_heads, frequencies, positions, position_bytes,
                 position_stride_b, position_stride_n, magnitude, dtype, batch, n, head_dim, rotary_dim, interleaved, inverse,
                 static_cast<cudaStream_t>(stream));
