@@ -2,6 +2,7 @@
 // argument validation and host orchestration.  Stream-ordered like api.cu; nothing allocates device memory or synchronises.
 #include <algorithm>
 
+#include "decode.cuh"
 #include "kernels.cuh"
 
 using namespace elsa;
@@ -10,6 +11,67 @@ namespace {
 
 bool inputs_ok(const void* p, int heads, int n, int head_dim, int batch, int dtype) {
   return p && heads > 0 && n > 0 && batch > 0 && head_dim > 0 && dtype_ok(dtype);
+}
+
+// a tensor-core kernel's wait that gave up is reported by every later call that would launch one (api.cu)
+int device_status_ok() {
+  volatile int* host = nullptr;
+  const int rc = device_status_word(nullptr, &host);
+  if (rc != ELSA_OK) return rc;
+  return *host != 0 ? ELSA_ERR_DEVICE_TIMEOUT : ELSA_OK;
+}
+
+// keys of one split: enough blocks for four waves of two on an SM, in multiples of 64 keys
+int split_width(int64_t blocks_of_one_split, int n_keys) {
+  const int64_t wanted = std::max<int64_t>(1, 8ll * sm_count() / blocks_of_one_split);
+  const int64_t width = align_up(cdiv64(n_keys, wanted), 64);
+  return static_cast<int>(std::max<int64_t>(64, std::min<int64_t>(width, 1024)));
+}
+
+// ---- attention over a shared prefix ------------------------------------------------------------------------------------
+struct PrefixPlan {
+  bool fold;                    // the prefix on the 128- and 256-row tensor-core fold (fold_tc.cu, fold_tcw.cu)
+  int prefix_width, prefix_parts, own_width, own_parts;
+  int64_t rows, q_bytes, mz_bytes, s_bytes;
+  int64_t bytes() const { return q_bytes + 2 * mz_bytes + s_bytes; }
+};
+
+// More rows for each key head than two 16-row tiles: the split kernel would read the prefix once for each tile.
+constexpr int kFoldRows = 32;
+
+int plan_prefix(int dtype, int batch, int heads, int kv_heads, int nq, int head_dim, int n_prefix, int n_own, PrefixPlan* pl) {
+  if (!dtype_ok(dtype) || batch < 1 || heads < 1 || kv_heads < 1 || heads % kv_heads || nq < 1 || head_dim < 1 || n_prefix < 0 || n_own < 0)
+    return ELSA_ERR_INVALID_ARGUMENT;
+  if (head_dim > 128) return ELSA_ERR_UNSUPPORTED;
+  const int64_t rows = static_cast<int64_t>(batch) * (heads / kv_heads) * nq;
+  if (rows * heads > 0x3fffffff || kv_heads > 65535 || n_prefix > 0x3fffffff || n_own > 0x3fffffff) return ELSA_ERR_UNSUPPORTED;
+  pl->rows = rows;
+  pl->fold = rows > kFoldRows && n_prefix >= 128 && (fold_tc_supported(dtype, head_dim, false) || fold_tcw_supported(dtype, head_dim, false));
+  pl->prefix_width = pl->prefix_parts = pl->own_width = pl->own_parts = 0;
+  if (n_own > 0) {
+    pl->own_width = split_width(static_cast<int64_t>(batch) * kv_heads * cdiv64(heads / kv_heads * nq, 16), n_own);
+    pl->own_parts = static_cast<int>(cdiv64(n_own, pl->own_width));
+  }
+  if (pl->fold) {
+    // one CTA for each row tile, key head and part, one CTA on an SM: waves x (key tiles of a part + what a CTA costs besides, about
+    // four of them)
+    const int tile = head_dim <= 64 ? 256 : 128;
+    const int64_t ctas = cdiv64(rows, tile) * kv_heads, tiles = cdiv64(n_prefix, 128);
+    int64_t best = 0, best_cost = 0;
+    for (int64_t parts = 1; parts <= std::min<int64_t>(tiles, 64); ++parts) {
+      const int64_t per = cdiv64(tiles, parts), cost = cdiv64(ctas * cdiv64(tiles, per), sm_count()) * (per + 4);
+      if (best == 0 || cost < best_cost) { best = per; best_cost = cost; }
+    }
+    pl->prefix_width = static_cast<int>(best * 128);
+  } else if (n_prefix > 0) {
+    pl->prefix_width = split_width(kv_heads * cdiv64(rows, 16), n_prefix);
+  }
+  if (n_prefix > 0) pl->prefix_parts = static_cast<int>(cdiv64(n_prefix, pl->prefix_width));
+  const int64_t summaries = static_cast<int64_t>(pl->prefix_parts + pl->own_parts) * kv_heads * rows;
+  pl->q_bytes = pl->fold ? align_up(rows * kv_heads * head_dim * 2, 256) : 0;
+  pl->mz_bytes = align_up(summaries * 4, 256);
+  pl->s_bytes = align_up(summaries * head_dim * 4, 256);
+  return ELSA_OK;
 }
 
 }  // namespace
@@ -30,4 +92,64 @@ extern "C" int elsa_rotary(const void* q, void* q_out, const int64_t* q_strides,
   return rotary(q, q_out, q_strides, q_heads, k, k_out, k_strides, k_heads, frequencies, positions, position_bytes,
                 position_stride_b, position_stride_n, magnitude, dtype, batch, n, head_dim, rotary_dim, interleaved, inverse,
                 static_cast<cudaStream_t>(stream));
+}
+
+extern "C" int64_t elsa_shared_prefix_workspace_bytes(int dtype, int batch, int heads, int kv_heads, int nq, int head_dim, int n_prefix,
+                                                      int n_own) {
+  PrefixPlan pl;
+  return plan_prefix(dtype, batch, heads, kv_heads, nq, head_dim, n_prefix, n_own, &pl) == ELSA_OK ? pl.bytes() : -1;
+}
+
+extern "C" int elsa_shared_prefix_attention(const void* q, const void* k_prefix, const void* v_prefix, const void* k, const void* v,
+                                            void* out, const int64_t* strides, const int* lengths, void* workspace,
+                                            int64_t workspace_bytes, int dtype, int batch, int heads, int kv_heads, int nq,
+                                            int head_dim, int n_prefix, int n_own, double scale, void* stream) {
+  PrefixPlan pl;
+  int rc = plan_prefix(dtype, batch, heads, kv_heads, nq, head_dim, n_prefix, n_own, &pl);
+  if (rc != ELSA_OK) return rc;
+  if (!q || !out || !strides || (n_prefix > 0 && (!k_prefix || !v_prefix)) || (n_own > 0 && (!k || !v))) return ELSA_ERR_INVALID_ARGUMENT;
+  if (pl.bytes() > 0 && (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 255u) || workspace_bytes < pl.bytes())) return ELSA_ERR_WORKSPACE;
+  auto st = static_cast<cudaStream_t>(stream);
+  char* ws = static_cast<char*>(workspace);
+  DecodeParams p{};
+  p.q = q; p.qs = Strides{strides[0], strides[1], strides[2]};
+  p.batch = batch; p.heads = heads; p.kv_heads = kv_heads; p.nq = nq; p.head_dim = p.v_dim = head_dim; p.maps = 1;
+  p.scale_log2 = static_cast<float>(scale * 1.4426950408889634);
+  p.m = reinterpret_cast<float*>(ws + pl.q_bytes);
+  p.z = reinterpret_cast<float*>(ws + pl.q_bytes + pl.mz_bytes);
+  p.s = reinterpret_cast<float*>(ws + pl.q_bytes + 2 * pl.mz_bytes);
+  p.out = out; p.os = Strides{strides[13], strides[14], strides[15]};
+  const Strides kps{0, strides[3], strides[4]}, vps{0, strides[5], strides[6]};
+  bool fold = pl.fold;
+  if (fold) {
+    // what tensor maps ask of the prefix; another layout goes through the split kernel with the same parts
+    fold = !((kps.h | kps.r | vps.h | vps.r) & 7) && kps.r >= head_dim && vps.r >= head_dim && (kv_heads == 1 || (kps.h > 0 && vps.h > 0)) &&
+           !((reinterpret_cast<uintptr_t>(k_prefix) | reinterpret_cast<uintptr_t>(v_prefix)) & 15u);
+  }
+  if (fold) {
+    if ((rc = device_status_ok()) != ELSA_OK) return rc;
+    if ((rc = decode_pack_q(p, ws, st)) != ELSA_OK) return rc;
+    FoldParams f{};
+    f.q = ws; f.k = k_prefix; f.v = v_prefix;
+    f.qs = contiguous_strides(kv_heads, pl.rows, head_dim); f.ks = kps; f.vs = vps;
+    f.m = p.m; f.z = p.z; f.s = p.s;
+    f.heads = f.bh = kv_heads; f.n_ctx = f.q_len = static_cast<int>(pl.rows); f.head_dim = head_dim;
+    f.part_width = pl.prefix_width; f.n_parts = pl.prefix_parts; f.n_keys = n_prefix;
+    f.summary_dtype = ELSA_F32;
+    f.scale = static_cast<float>(scale); f.scale_log2 = p.scale_log2;
+    rc = head_dim <= 64 ? fold_tc(f, dtype, st) : fold_tcw(f, dtype, st);
+    if (rc != ELSA_OK) return rc;
+  } else if (n_prefix > 0) {
+    DecodeSegment& s = p.seg[p.n_segs++];
+    s.k = k_prefix; s.v = v_prefix; s.ks = kps; s.vs = vps; s.n_keys = n_prefix; s.shared = 1;
+    s.split_width = pl.prefix_width; s.n_splits = pl.prefix_parts; s.first_part = 0;
+  }
+  if (n_own > 0) {
+    DecodeSegment& s = p.seg[p.n_segs++];
+    s.k = k; s.v = v; s.ks = Strides{strides[7], strides[8], strides[9]}; s.vs = Strides{strides[10], strides[11], strides[12]};
+    s.lengths = lengths; s.n_keys = n_own; s.causal = 1;
+    s.split_width = pl.own_width; s.n_splits = pl.own_parts; s.first_part = pl.prefix_parts;
+  }
+  if ((rc = decode_split(p, dtype, st)) != ELSA_OK) return rc;
+  return decode_merge(p, pl.prefix_parts + pl.own_parts, dtype, st);
 }

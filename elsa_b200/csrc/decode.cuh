@@ -1,0 +1,48 @@
+// Attention of few query rows over long key caches, split along the keys: the per-split (m, z, s) summaries (decode.cu) and
+// their merge.  Used by the shared-prefix attention (one softmax map) and by the single-token form of the differential
+// attention (two maps over one value cache).
+#pragma once
+
+#include "kernels.cuh"
+
+namespace elsa {
+
+// One key cache.  shared: [kv heads, n_keys, .] for all sequences (batch strides unused), every query sees every key.
+// Otherwise [batch, kv heads, n_keys, .]: sequence b has lengths[b] keys (null: n_keys) and, where causal, its query i of nq
+// sees the first lengths[b] - nq + i + 1 of them.  Keys from lengths[b] on are never read.
+struct DecodeSegment {
+  const void* k; const void* v;
+  Strides ks, vs;                       // head axis of k: maps * kv heads, of v: kv heads
+  const int* lengths;
+  int n_keys, causal, shared;
+  int split_width, n_splits, first_part;
+  int row_tiles;                        // set by the launcher
+  int64_t blocks;                       // set by the launcher
+};
+
+// Rows are numbered within their kv head: row = (b * group + query head within the group) * nq + i, `rows` of them.
+// Summaries: m, z [part][kv head][row][map], s [part][kv head][row][map][v_dim], fp32; m in the log2 domain.
+struct DecodeParams {
+  const void* q; Strides qs;            // [batch, maps * heads, nq, head_dim]
+  int batch, heads, kv_heads, nq, head_dim, v_dim, maps;
+  float scale_log2;
+  DecodeSegment seg[2]; int n_segs;
+  float* m; float* z; float* s;
+  // the merge
+  const float* lam;                     // maps == 2: out = s1 / z1 - lam[h] s2 / z2, one value for each head or for all (lam_stride 0)
+  int lam_stride;
+  void* out; Strides os;                // [batch, heads, nq, v_dim]
+};
+
+__host__ __device__ inline int64_t decode_rows(const DecodeParams& p) { return static_cast<int64_t>(p.batch) * (p.heads / p.kv_heads) * p.nq; }
+
+// whether the tensor-core kernel takes this: 16-bit types, rows on 16-byte boundaries, head and value dims it has
+bool decode_mma_ok(const DecodeParams& p, int dtype);
+// summaries of all segments in one launch; parts that begin beyond a sequence's keys are not written
+int decode_split(DecodeParams& p, int dtype, cudaStream_t st);
+// q of 16-bit elements (one map) as [kv head][row][head_dim]
+int decode_pack_q(const DecodeParams& p, void* packed, cudaStream_t st);
+// all parts of a row merged (of a segment that is not shared: those that begin before the sequence's last key)
+int decode_merge(const DecodeParams& p, int n_parts, int dtype, cudaStream_t st);
+
+}  // namespace elsa

@@ -355,6 +355,21 @@ int elsa_rotary(const void* q, void* q_out, const int64_t* q_strides, int q_head
                 int64_t position_stride_b, int64_t position_stride_n, double magnitude, int dtype, int batch, int n,
                 int head_dim, int rotary_dim, int interleaved, int inverse, void* stream);
 
+/* Attention of a batch that shares a long prefix: query i of sequence b sees the whole prefix and, of the sequence's own cache, the
+ * first lengths[b] - nq + i + 1 keys (its own tokens are the last nq of lengths[b]; none where that is not positive).  The prefix's keys and values are
+ * read for the batch, not for each sequence.  A query that sees no key at all gets zeros.
+ * q, out: [batch, heads, nq, head_dim]; k_prefix, v_prefix: [kv_heads, n_prefix, head_dim]; k, v: [batch, kv_heads, n_own, head_dim];
+ * query head h reads kv head h / (heads / kv_heads).  lengths: 32-bit integers on the device, clamped to 0 .. n_own; NULL: n_own.
+ * `strides` = element strides, in this order: q {b, h, r}, k_prefix {h, r}, v_prefix {h, r}, k {b, h, r}, v {b, h, r}, out {b, h, r}; the
+ * elements of a row are contiguous.  head_dim <= 128.  16-bit inputs whose rows start on 16-byte boundaries run on the tensor
+ * cores.  n_prefix or n_own may be 0 (then its pointers are not looked at).
+ * workspace (256-byte aligned): elsa_shared_prefix_workspace_bytes; -1 for sizes that the call would refuse. */
+int64_t elsa_shared_prefix_workspace_bytes(int dtype, int batch, int heads, int kv_heads, int nq, int head_dim, int n_prefix, int n_own);
+int elsa_shared_prefix_attention(const void* q, const void* k_prefix, const void* v_prefix, const void* k, const void* v, void* out,
+                                 const int64_t* strides, const int* lengths, void* workspace, int64_t workspace_bytes, int dtype,
+                                 int batch, int heads, int kv_heads, int nq, int head_dim, int n_prefix, int n_own, double scale,
+                                 void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -85,3 +85,34 @@ def test_rotary_abi_refuses_before_any_launch(lib):
     assert call(r=65) == 2 and call(r=0) == 2 and call(d=64, r=128) == 2 and call(d=2048) == 2 and call(d=512, r=512) == 2
     assert call(pos=64, pos_bytes=0) == 1 and call(pos=None, pos_bytes=8) == 1 and call(pos=64, pos_bytes=2) == 1
     assert call(q=64, q_out=64, strides=other) == 1
+
+
+# ---- attention over a shared prefix --------------------------------------------------------------------------------
+def test_shared_prefix_refuses_before_any_launch(lib):
+    import ctypes
+    q, kp, k = torch.zeros(2, 4, 1, 16), torch.zeros(2, 5, 16), torch.zeros(2, 2, 3, 16)
+    with pytest.raises(ValueError, match="CUDA"):
+        E.shared_prefix_attention(q, kp, kp, k, k)
+    with pytest.raises(ValueError, match="multiple"):
+        E.shared_prefix_attention(q[:, :3], kp, kp, k, k)
+    size = lib.elsa_shared_prefix_workspace_bytes
+    assert size(1, 2, 4, 2, 1, 64, 100, 50) > 0 and size(1, 2, 4, 2, 1, 64, 0, 0) == 0
+    for bad in ((9, 2, 4, 2, 1, 64, 100, 50), (1, 0, 4, 2, 1, 64, 100, 50), (1, 2, 4, 3, 1, 64, 100, 50), (1, 2, 4, 2, 0, 64, 100, 50),
+                (1, 2, 4, 2, 1, 129, 100, 50), (1, 2, 4, 2, 1, 64, -1, 50), (1, 1 << 28, 4, 2, 1, 64, 100, 50)):
+        assert size(*bad) == -1
+    st = (ctypes.c_int64 * 16)(*([64] * 16))
+
+    def call(q=256, kp=256, k=256, out=256, strides=st, ws=256, nbytes=1 << 40, dtype=1, batch=2, heads=4, kv=2):
+        return lib.elsa_shared_prefix_attention(q, kp, kp, k, k, out, strides, None, ws, nbytes, dtype, batch, heads, kv, 1, 64, 100, 50, 0.125, None)
+
+    assert call(q=None) == 1 and call(kp=None) == 1 and call(k=None) == 1 and call(out=None) == 1 and call(strides=None) == 1
+    assert call(dtype=5) == 1 and call(kv=3) == 1 and call(batch=-1) == 1
+    assert call(ws=None) == 4 and call(ws=128) == 4 and call(nbytes=1000) == 4
+
+
+def test_shared_prefix_splits_cover_every_key(lib):
+    """Summaries for every part, whatever the sizes (the workspace holds m, z and D sums of each row and part)."""
+    for batch, heads, kv, nq, d, p, s in ((1, 1, 1, 1, 64, 1, 1), (256, 32, 8, 1, 128, 32768, 2048), (8, 8, 8, 1, 64, 512, 128), (24, 12, 3, 5, 96, 4097, 333)):
+        rows = batch * heads // kv * nq
+        least = 2 * kv * rows * (d + 2) * 4
+        assert lib.elsa_shared_prefix_workspace_bytes(2, batch, heads, kv, nq, d, p, s) >= least
