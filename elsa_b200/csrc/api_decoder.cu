@@ -21,9 +21,12 @@ int device_status_ok() {
   return *host != 0 ? ELSA_ERR_DEVICE_TIMEOUT : ELSA_OK;
 }
 
-// keys of one split: enough blocks for four waves of two on an SM, in multiples of 64 keys
+// Keys of one split.  A block costs about 4 us besides its keys (launch, first loads, merge of its warps), so there are as few
+// splits as give two waves of two blocks on an SM, whose second wave evens out caches of different lengths.  Measured, bf16, head
+// dim 128: 256 x 8 caches of up to 2048 keys 174 us at 1024 keys a split, 238 at 256, 550 at 64; 64 x 8 of up to 1024 keys 33 us at
+// 512 or 1024, 49 at 128; 24 x 3 of up to 333 keys 8.9 us at 512, 9.3 at 128, 13.3 at 64.
 int split_width(int64_t blocks_of_one_split, int n_keys) {
-  const int64_t wanted = std::max<int64_t>(1, 8ll * sm_count() / blocks_of_one_split);
+  const int64_t wanted = std::max<int64_t>(1, 4ll * sm_count() / blocks_of_one_split);
   const int64_t width = align_up(cdiv64(n_keys, wanted), 64);
   return static_cast<int>(std::max<int64_t>(64, std::min<int64_t>(width, 1024)));
 }

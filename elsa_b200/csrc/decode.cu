@@ -181,7 +181,8 @@ split_mma_kernel(const DecodeParams p) {
 
   for (int it = 0; it < mine; ++it) {
     asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 2) : "memory");
-    __syncwarp();                                       // every lane's copies of this stage are there
+    __syncwarp();                                       // every lane's copies of this stage are there, and the stage before it has been read
+    copy(it + kStages - 1);                             // over that one: two stages are on their way while this one is used
     const uint32_t st = ring + (it % kStages) * Tile::kStage;
     const int key0 = w.k0 + (warp + it * kMmaWarps) * kMmaKeys + quad * 2;
     uint32_t pf[MAPS][4];
@@ -245,8 +246,6 @@ split_mma_kernel(const DecodeParams p) {
         mma16816<T>(o[m][2 * n + 1], pf[m], vf[2], vf[3]);
       }
     }
-    __syncwarp();                                       // every lane has read the stage that the next copy overwrites
-    copy(it + kStages - 1);
   }
   asm volatile("cp.async.wait_group 0;" ::: "memory");
   __syncthreads();                                      // the ring becomes the merge buffer
@@ -260,6 +259,7 @@ split_mma_kernel(const DecodeParams p) {
     for (int h = 0; h < 2; ++h) {
       z[m][h] += __shfl_xor_sync(0xffffffffu, z[m][h], 1);
       z[m][h] += __shfl_xor_sync(0xffffffffu, z[m][h], 2);
+      if (qrow + 8 * h >= w.n_rows) continue;
       float* dst = slot(warp, m, qrow + 8 * h);
 #pragma unroll
       for (int n = 0; n < VP / 8; ++n) *reinterpret_cast<float2*>(dst + n * 8 + quad * 2) = make_float2(o[m][n][2 * h], o[m][n][2 * h + 1]);
@@ -416,81 +416,110 @@ split_simt_kernel(const DecodeParams p) {
 }
 
 // ---- merge ------------------------------------------------------------------------------------------------------------
-// A warp per (kv head, row): the weights of the parts first (a lane per part, 32 parts at a time), then their sums, a lane per
-// value column.  A row that sees no key (every z = 0) is zeros.
-template <typename T, int MAPS>
+// A warp per (kv head, row): the weights of the parts first (a lane per part, 32 parts at a time), then their sums, VEC value
+// columns of each lane (VEC 4 where a row of sums is a multiple of 16 bytes), eight parts' loads in flight.  A row that sees no
+// key (every z = 0) is zeros; a NaN stays one.
+template <typename T, int MAPS, int VEC>
 __global__ void __launch_bounds__(128)
 merge_kernel(const DecodeParams p, int n_parts) {
+  constexpr int kAhead = 8, kCols = 4 / VEC;            // column groups of a lane: VEC (lane + 32 e) ..., at most 128 columns
   const int64_t rows = decode_rows(p);
-  const int64_t i = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 5);
+  const int i = blockIdx.x * 4 + (threadIdx.x >> 5);
   const int lane = threadIdx.x & 31;
   if (i >= rows * p.kv_heads) return;
-  const int g = static_cast<int>(i / rows), row = static_cast<int>(i - g * rows);
+  const int g = i / static_cast<int>(rows), row = i - g * static_cast<int>(rows);
   const int group = p.heads / p.kv_heads, per = group * p.nq;
   const int b = row / per, r = row - b * per, gi = r / p.nq, t = r - gi * p.nq, h = g * group + gi;
-  auto written = [&](int part) {                        // was this part's summary of this row written?
-    for (int s = 0; s < p.n_segs; ++s) {
+  // parts [from, to) of a segment whose splits begin behind the sequence's last key were not written
+  int from[2] = {0, 0}, to[2] = {0, 0};
+#pragma unroll
+  for (int s = 0; s < 2; ++s)
+    if (s < p.n_segs) {
       const DecodeSegment& sg = p.seg[s];
-      const int at = part - sg.first_part;
-      if (at < 0 || at >= sg.n_splits) continue;
-      const int len = sg.shared || !sg.lengths ? sg.n_keys : min(sg.n_keys, sg.lengths[b]);
-      return static_cast<int64_t>(at) * sg.split_width < len;
+      const int len = sg.shared || !sg.lengths ? sg.n_keys : max(0, min(sg.n_keys, sg.lengths[b]));
+      from[s] = sg.first_part + (len + sg.split_width - 1) / sg.split_width;
+      to[s] = sg.first_part + sg.n_splits;
     }
-    return true;                                        // (a part of another kernel: always)
-  };
-  auto at = [&](int part, int m) { return ((static_cast<int64_t>(part) * p.kv_heads + g) * rows + row) * MAPS + m; };
-  float total[4] = {0.f, 0.f, 0.f, 0.f};                // value columns lane + 32 {0..3}
+  auto written = [&](int part) { return !(part >= from[0] && part < to[0]) && !(part >= from[1] && part < to[1]); };
+  const int64_t step = static_cast<int64_t>(p.kv_heads) * rows * MAPS;      // from one part to the next
+  const int64_t first = (static_cast<int64_t>(g) * rows + row) * MAPS;
+  float total[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
   for (int m = 0; m < MAPS; ++m) {
-    float top = -CUDART_INF_F;
-    for (int p0 = lane; p0 < n_parts; p0 += 32)
-      if (written(p0)) top = fmaxf(top, p.m[at(p0, m)]);
-#pragma unroll
-    for (int x = 16; x > 0; x >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
-    float zs = 0.f, acc[4] = {0.f, 0.f, 0.f, 0.f};
+    const float* pm = p.m + first + m;
+    const float* pz = p.z + first + m;
+    const float* ps = p.s + (first + m) * p.v_dim + lane * VEC;
+    float top = -CUDART_INF_F, zs = 0.f, acc[4] = {0.f, 0.f, 0.f, 0.f};
     for (int p0 = 0; p0 < n_parts; p0 += 32) {
-      float f = 0.f;
+      float m_part = -CUDART_INF_F, z_part = 0.f;
       if (p0 + lane < n_parts && written(p0 + lane)) {
-        const int64_t a = at(p0 + lane, m);
-        const float zp = p.z[a];
-        if (zp != 0.f) {                                // (a NaN stays one)
-          f = exp2f(p.m[a] - top);
-          zs += f * zp;
-        }
+        m_part = pm[(p0 + lane) * step];
+        z_part = pz[(p0 + lane) * step];
       }
-      const int n = min(32, n_parts - p0);
-      for (int j = 0; j < n; ++j) {
-        const float fj = __shfl_sync(0xffffffffu, f, j);
-        if (fj == 0.f) continue;                        // (warp-uniform)
-        const float* src = p.s + at(p0 + j, m) * p.v_dim;
+      float best = m_part;
 #pragma unroll
-        for (int e = 0; e < 4; ++e)
-          if (lane + 32 * e < p.v_dim) acc[e] = fmaf(fj, src[lane + 32 * e], acc[e]);
+      for (int x = 16; x > 0; x >>= 1) best = fmaxf(best, __shfl_xor_sync(0xffffffffu, best, x));
+      if (best > top) {                                 // (more than 32 parts: what came before is rescaled)
+        const float alpha = exp2f(top - best);
+        zs *= alpha;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) acc[e] *= alpha;
+        top = best;
+      }
+      const float f = z_part != 0.f ? exp2f(m_part - top) : 0.f;
+      zs += z_part != 0.f ? f * z_part : 0.f;
+      const int n = min(32, n_parts - p0);
+      for (int j0 = 0; j0 < n; j0 += kAhead) {
+        float x[kAhead][4];
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u) {
+          const bool take = __shfl_sync(0xffffffffu, f, j0 + u) != 0.f;       // (lanes beyond n have f = 0)
+          const float* src = ps + (p0 + j0 + u) * step * p.v_dim;
+          if (VEC == 4) {
+            const float4 v = take && lane * 4 < p.v_dim ? *reinterpret_cast<const float4*>(src) : make_float4(0.f, 0.f, 0.f, 0.f);
+            x[u][0] = v.x; x[u][1] = v.y; x[u][2] = v.z; x[u][3] = v.w;
+          } else {
+#pragma unroll
+            for (int e = 0; e < kCols; ++e) x[u][e] = take && lane + 32 * e < p.v_dim ? src[32 * e] : 0.f;
+          }
+        }
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u) {
+          const float fj = __shfl_sync(0xffffffffu, f, j0 + u);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) acc[e] = fmaf(fj, x[u][e], acc[e]);
+        }
       }
     }
 #pragma unroll
     for (int x = 16; x > 0; x >>= 1) zs += __shfl_xor_sync(0xffffffffu, zs, x);
     float f = 1.f / zs;
-    if (MAPS == 2 && m == 1) f *= -p.lam[static_cast<int64_t>(h) * p.lam_stride];
+    if (MAPS == 2 && m == 1) {
+      const int64_t at = static_cast<int64_t>(h) * p.lam_stride;
+      f *= -(p.lam_dtype == ELSA_F32 ? static_cast<const float*>(p.lam)[at] : p.lam_dtype == ELSA_F16 ? to_f32(static_cast<const __half*>(p.lam)[at])
+                                                                                                    : to_f32(static_cast<const __nv_bfloat16*>(p.lam)[at]));
+    }
 #pragma unroll
     for (int e = 0; e < 4; ++e) total[e] += zs != 0.f ? f * acc[e] : 0.f;
   }
   T* dst = static_cast<T*>(p.out) + b * p.os.b + h * p.os.h + t * p.os.r;
 #pragma unroll
-  for (int e = 0; e < 4; ++e)
-    if (lane + 32 * e < p.v_dim) dst[lane + 32 * e] = from_f32<T>(total[e]);
+  for (int e = 0; e < 4; ++e) {
+    const int col = VEC == 4 ? lane * 4 + e : lane + 32 * e;
+    if (col < p.v_dim) dst[col] = from_f32<T>(total[e]);
+  }
 }
 
-// q as [kv head][row][head_dim]
-template <typename T>
+// q as [kv head][row][head_dim], E the elements of one access
+template <typename E>
 __global__ void __launch_bounds__(256)
-pack_q_kernel(const DecodeParams p, T* packed) {
-  const int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x, rows = decode_rows(p);
-  if (i >= rows * p.kv_heads * p.head_dim) return;
-  const int col = static_cast<int>(i % p.head_dim);
-  const int64_t gr = i / p.head_dim;
-  const int g = static_cast<int>(gr / rows), row = static_cast<int>(gr - g * rows);
-  packed[i] = static_cast<const T*>(p.q)[q_offset(p, g, row, 0) + col];
+pack_q_kernel(const DecodeParams p, E* packed, int row_elements) {
+  const int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
+  const int rows = static_cast<int>(decode_rows(p));
+  if (i >= static_cast<int64_t>(rows) * p.kv_heads * row_elements) return;
+  const int gr = static_cast<int>(i / row_elements), col = static_cast<int>(i - static_cast<int64_t>(gr) * row_elements);
+  const int g = gr / rows, row = gr - g * rows;
+  packed[i] = reinterpret_cast<const E*>(static_cast<const __half*>(p.q) + q_offset(p, g, row, 0))[col];
 }
 
 template <typename T, int MAPS, int DP, int VP>
@@ -555,23 +584,32 @@ int decode_split(DecodeParams& p, int dtype, cudaStream_t st) {
 }
 
 int decode_pack_q(const DecodeParams& p, void* packed, cudaStream_t st) {
-  const int64_t blocks = cdiv64(decode_rows(p) * p.kv_heads * p.head_dim, 256);
-  if (blocks > 0x7fffffffll || p.maps != 1) return ELSA_ERR_UNSUPPORTED;
+  if (p.maps != 1) return ELSA_ERR_UNSUPPORTED;
+  const bool wide = p.head_dim % 8 == 0 && !((p.qs.b | p.qs.h | p.qs.r) & 7) && !(reinterpret_cast<uintptr_t>(p.q) & 15u);
+  const int row_elements = wide ? p.head_dim / 8 : p.head_dim;
+  const int64_t blocks = cdiv64(decode_rows(p) * p.kv_heads * row_elements, 256);
+  if (blocks > 0x7fffffffll) return ELSA_ERR_UNSUPPORTED;
   // (16-bit elements are moved, not looked at)
-  pack_q_kernel<__half><<<static_cast<unsigned>(blocks), 256, 0, st>>>(p, static_cast<__half*>(packed));
+  if (wide) pack_q_kernel<uint4><<<static_cast<unsigned>(blocks), 256, 0, st>>>(p, static_cast<uint4*>(packed), row_elements);
+  else pack_q_kernel<uint16_t><<<static_cast<unsigned>(blocks), 256, 0, st>>>(p, static_cast<uint16_t*>(packed), row_elements);
+  ELSA_LAUNCH_CHECK();
+  return ELSA_OK;
+}
+
+template <typename T>
+static int merge_t(const DecodeParams& p, int n_parts, unsigned grid, cudaStream_t st) {
+  const bool vec = p.v_dim % 4 == 0;                    // (the sums start on a 256-byte boundary)
+  const auto kernel = p.maps == 2 ? (vec ? &merge_kernel<T, 2, 4> : &merge_kernel<T, 2, 1>) : (vec ? &merge_kernel<T, 1, 4> : &merge_kernel<T, 1, 1>);
+  kernel<<<grid, 128, 0, st>>>(p, n_parts);
   ELSA_LAUNCH_CHECK();
   return ELSA_OK;
 }
 
 int decode_merge(const DecodeParams& p, int n_parts, int dtype, cudaStream_t st) {
-  const int64_t blocks = cdiv64(decode_rows(p) * p.kv_heads, 4);
-  if (blocks > 0x7fffffffll) return ELSA_ERR_UNSUPPORTED;
-  const unsigned grid = static_cast<unsigned>(blocks);
-  if (dtype == ELSA_F32) (p.maps == 2 ? &merge_kernel<float, 2> : &merge_kernel<float, 1>)<<<grid, 128, 0, st>>>(p, n_parts);
-  else if (dtype == ELSA_F16) (p.maps == 2 ? &merge_kernel<__half, 2> : &merge_kernel<__half, 1>)<<<grid, 128, 0, st>>>(p, n_parts);
-  else (p.maps == 2 ? &merge_kernel<__nv_bfloat16, 2> : &merge_kernel<__nv_bfloat16, 1>)<<<grid, 128, 0, st>>>(p, n_parts);
-  ELSA_LAUNCH_CHECK();
-  return ELSA_OK;
+  if (decode_rows(p) * p.kv_heads > 0x3fffffff) return ELSA_ERR_UNSUPPORTED;
+  const unsigned grid = static_cast<unsigned>(cdiv64(decode_rows(p) * p.kv_heads, 4));
+  if (dtype == ELSA_F32) return merge_t<float>(p, n_parts, grid, st);
+  return dtype == ELSA_F16 ? merge_t<__half>(p, n_parts, grid, st) : merge_t<__nv_bfloat16>(p, n_parts, grid, st);
 }
 
 }  // namespace elsa

@@ -29,8 +29,7 @@ struct DecodeParams {
   DecodeSegment seg[2]; int n_segs;
   float* m; float* z; float* s;
   // the merge
-  const float* lam;                     // maps == 2: out = s1 / z1 - lam[h] s2 / z2, one value for each head or for all (lam_stride 0)
-  int lam_stride;
+  const void* lam; int lam_dtype, lam_stride;   // maps == 2: out = s1 / z1 - lam[h] s2 / z2, a value for each head or for all (lam_stride 0)
   void* out; Strides os;                // [batch, heads, nq, v_dim]
 };
 
