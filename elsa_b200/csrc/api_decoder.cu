@@ -3,6 +3,7 @@
 #include <algorithm>
 
 #include "decode.cuh"
+#include "diff.cuh"
 #include "kernels.cuh"
 
 using namespace elsa;
@@ -77,6 +78,49 @@ int plan_prefix(int dtype, int batch, int heads, int kv_heads, int nq, int head_
   return ELSA_OK;
 }
 
+// ---- differential attention -------------------------------------------------------------------------------------------
+struct DiffPlan {
+  bool tensor_tiles;            // the 128-row tensor-core kernels by sizes (diff_tc.cu); else the split kernels (decode.cu)
+  int split_width, parts;       // of the split kernels
+  int64_t mz_bytes, s_bytes;
+  int64_t bytes() const { return 2 * mz_bytes + s_bytes; }
+};
+
+// Up to four 16-row tiles for each key head the split kernel, which works on keys side by side, is ahead of one CTA that walks over
+// them in 128-row tiles.
+constexpr int kSplitRows = 64;
+
+int plan_diff(int dtype, int batch, int heads, int kv_heads, int nq, int nk, int head_dim, int v_dim, DiffPlan* pl) {
+  if (!dtype_ok(dtype) || batch < 1 || heads < 1 || kv_heads < 1 || heads % kv_heads || nq < 1 || nk < 0 || head_dim < 1 || v_dim < 1)
+    return ELSA_ERR_INVALID_ARGUMENT;
+  if (head_dim > 128 || v_dim > 128) return ELSA_ERR_UNSUPPORTED;
+  const int64_t rows_b = static_cast<int64_t>(heads / kv_heads) * nq, rows = rows_b * batch;
+  if (rows * kv_heads > 0x1fffffff || heads > 65535 || batch > 65535 || nk > 0x3fffffff || nq > 0x3fffffff) return ELSA_ERR_UNSUPPORTED;
+  pl->tensor_tiles = rows_b > kSplitRows && diff_tc_sizes(dtype, head_dim, v_dim);
+  pl->split_width = nk > 0 ? split_width(static_cast<int64_t>(batch) * kv_heads * cdiv64(rows_b, 16), nk) : 1;
+  pl->parts = static_cast<int>(cdiv64(nk, pl->split_width));
+  const int64_t summaries = 2 * static_cast<int64_t>(pl->parts) * kv_heads * rows;
+  pl->mz_bytes = align_up(summaries * 4, 256);
+  pl->s_bytes = align_up(summaries * v_dim * 4, 256);
+  return ELSA_OK;
+}
+
+DiffParams diff_params(const void* q, const void* k, const void* v, const void* lam, int lam_dtype, int lam_stride, const int64_t* st,
+                       int batch, int heads, int kv_heads, int nq, int nk, int head_dim, int v_dim, int is_causal, double scale) {
+  DiffParams p{};
+  p.q = q; p.k = k; p.v = v;
+  p.qs = Strides{st[0], st[1], st[2]}; p.ks = Strides{st[3], st[4], st[5]}; p.vs = Strides{st[6], st[7], st[8]};
+  p.lam = lam; p.lam_dtype = lam_dtype; p.lam_stride = lam_stride;
+  p.batch = batch; p.heads = heads; p.kv_heads = kv_heads; p.nq = nq; p.nk = nk; p.head_dim = head_dim; p.v_dim = v_dim; p.causal = is_causal;
+  p.scale = static_cast<float>(scale); p.scale_log2 = static_cast<float>(scale * 1.4426950408889634);
+  return p;
+}
+
+bool diff_inputs_in_tiles(const DiffParams& p) {
+  return diff_rows_ok(p.q, p.qs, p.head_dim, 2 * p.heads, p.batch) &&
+         (p.nk == 0 || (diff_rows_ok(p.k, p.ks, p.head_dim, 2 * p.kv_heads, p.batch) && diff_rows_ok(p.v, p.vs, p.v_dim, p.kv_heads, p.batch)));
+}
+
 }  // namespace
 
 extern "C" int elsa_rotary(const void* q, void* q_out, const int64_t* q_strides, int q_heads, const void* k, void* k_out,
@@ -110,7 +154,7 @@ extern "C" int elsa_shared_prefix_attention(const void* q, const void* k_prefix,
   PrefixPlan pl;
   int rc = plan_prefix(dtype, batch, heads, kv_heads, nq, head_dim, n_prefix, n_own, &pl);
   if (rc != ELSA_OK) return rc;
-  if (!q || !out || !strides || (n_prefix > 0 && (!k_prefix || !v_prefix)) || (n_own > 0 && (!k || !v))) return ELSA_ERR_INVALID_ARGUMENT;
+  if (!q || !out || !strides || (n_prefix > 0 && (!k_prefix || !v_prefix)) || (n_own > 0 && (!k || !v)) || !(scale > 0.0)) return ELSA_ERR_INVALID_ARGUMENT;
   if (pl.bytes() > 0 && (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 255u) || workspace_bytes < pl.bytes())) return ELSA_ERR_WORKSPACE;
   auto st = static_cast<cudaStream_t>(stream);
   char* ws = static_cast<char*>(workspace);
@@ -155,4 +199,44 @@ extern "C" int elsa_shared_prefix_attention(const void* q, const void* k_prefix,
   }
   if ((rc = decode_split(p, dtype, st)) != ELSA_OK) return rc;
   return decode_merge(p, pl.prefix_parts + pl.own_parts, dtype, st);
+}
+
+extern "C" int64_t elsa_differential_workspace_bytes(int dtype, int batch, int heads, int kv_heads, int nq, int nk, int head_dim, int v_dim) {
+  DiffPlan pl;
+  return plan_diff(dtype, batch, heads, kv_heads, nq, nk, head_dim, v_dim, &pl) == ELSA_OK ? pl.bytes() : -1;
+}
+
+extern "C" int elsa_differential_forward(const void* q, const void* k, const void* v, const void* lam, int lam_dtype, int lam_stride,
+                                         const int* lengths, void* out, const int64_t* strides, void* out2, float* lse, void* workspace,
+                                         int64_t workspace_bytes, int dtype, int batch, int heads, int kv_heads, int nq, int nk,
+                                         int head_dim, int v_dim, int is_causal, double scale, void* stream) {
+  DiffPlan pl;
+  int rc = plan_diff(dtype, batch, heads, kv_heads, nq, nk, head_dim, v_dim, &pl);
+  if (rc != ELSA_OK) return rc;
+  if (!q || !lam || !out || !strides || (nk > 0 && (!k || !v)) || !dtype_ok(lam_dtype) || !(scale > 0.0)) return ELSA_ERR_INVALID_ARGUMENT;
+  if (pl.bytes() > 0 && (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 255u) || workspace_bytes < pl.bytes())) return ELSA_ERR_WORKSPACE;
+  auto st = static_cast<cudaStream_t>(stream);
+  DiffParams d = diff_params(q, k, v, lam, lam_dtype, lam_stride, strides, batch, heads, kv_heads, nq, nk, head_dim, v_dim, is_causal, scale);
+  d.out = out; d.os = Strides{strides[9], strides[10], strides[11]};
+  d.out2 = out2; d.lse = lse;
+  // (what stands behind a sequence's last key must not be read: the tile kernel's loads are bounded by the tensors only)
+  if (pl.tensor_tiles && !lengths && diff_inputs_in_tiles(d) && diff_rows_ok(out, d.os, v_dim, heads, batch)) {
+    if ((rc = device_status_ok()) != ELSA_OK) return rc;
+    return diff_tc_fwd(d, dtype, st);
+  }
+  DecodeParams p{};
+  p.q = q; p.qs = d.qs;
+  p.batch = batch; p.heads = heads; p.kv_heads = kv_heads; p.nq = nq; p.head_dim = head_dim; p.v_dim = v_dim; p.maps = 2;
+  p.scale_log2 = d.scale_log2;
+  char* ws = static_cast<char*>(workspace);
+  p.m = reinterpret_cast<float*>(ws); p.z = reinterpret_cast<float*>(ws + pl.mz_bytes); p.s = reinterpret_cast<float*>(ws + 2 * pl.mz_bytes);
+  p.lam = lam; p.lam_dtype = lam_dtype; p.lam_stride = lam_stride;
+  p.out = out; p.os = d.os; p.out2 = out2; p.lse = lse;
+  if (nk > 0) {
+    DecodeSegment& s = p.seg[p.n_segs++];
+    s.k = k; s.v = v; s.ks = d.ks; s.vs = d.vs; s.lengths = lengths; s.n_keys = nk; s.causal = is_causal;
+    s.split_width = pl.split_width; s.n_splits = pl.parts;
+  }
+  if ((rc = decode_split(p, dtype, st)) != ELSA_OK) return rc;
+  return decode_merge(p, pl.parts, dtype, st);
 }

@@ -205,19 +205,19 @@ split_mma_kernel(const DecodeParams p) {
           s[n][e] = key < min(lim[e >> 1], w.k1) ? s[n][e] * c : -CUDART_INF_F;
           top[e >> 1] = fmaxf(top[e >> 1], s[n][e]);
         }
-      bool move = false;
+      bool move[2];
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         top[h] = fmaxf(top[h], __shfl_xor_sync(0xffffffffu, top[h], 1));
         top[h] = fmaxf(top[h], __shfl_xor_sync(0xffffffffu, top[h], 2));
-        move |= top[h] > m_ref[m][h] + kRescaleThreshold;
+        move[h] = top[h] > m_ref[m][h] + kRescaleThreshold;
       }
-      if (__any_sync(0xffffffffu, move)) {
+      if (__any_sync(0xffffffffu, move[0] || move[1])) {
         float alpha[2];
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-          const float m_new = fmaxf(m_ref[m][h], top[h]);
-          alpha[h] = m_new == -CUDART_INF_F ? 1.f : fast_exp2(m_ref[m][h] - m_new);
+          const float m_new = move[h] ? top[h] : m_ref[m][h];   // (a row's result does not depend on the rows beside it)
+          alpha[h] = move[h] ? fast_exp2(m_ref[m][h] - m_new) : 1.f;
           m_ref[m][h] = m_new;
           z[m][h] *= alpha[h];
         }
@@ -493,14 +493,30 @@ merge_kernel(const DecodeParams p, int n_parts) {
     }
 #pragma unroll
     for (int x = 16; x > 0; x >>= 1) zs += __shfl_xor_sync(0xffffffffu, zs, x);
-    float f = 1.f / zs;
-    if (MAPS == 2 && m == 1) {
-      const int64_t at = static_cast<int64_t>(h) * p.lam_stride;
-      f *= -(p.lam_dtype == ELSA_F32 ? static_cast<const float*>(p.lam)[at] : p.lam_dtype == ELSA_F16 ? to_f32(static_cast<const __half*>(p.lam)[at])
-                                                                                                    : to_f32(static_cast<const __nv_bfloat16*>(p.lam)[at]));
-    }
+    const float inv = 1.f / zs;
 #pragma unroll
-    for (int e = 0; e < 4; ++e) total[e] += zs != 0.f ? f * acc[e] : 0.f;
+    for (int e = 0; e < 4; ++e) acc[e] = zs != 0.f ? inv * acc[e] : 0.f;
+    if (MAPS == 1) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) total[e] = acc[e];
+    } else {
+      const int64_t ro = (static_cast<int64_t>(b) * p.heads + h) * p.nq + t;
+      if (p.lse && lane == 0) p.lse[m * (static_cast<int64_t>(p.batch) * p.heads * p.nq) + ro] = zs != 0.f ? top + log2f(zs) : -CUDART_INF_F;
+      if (m == 0) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) total[e] = acc[e];
+      } else {
+        const int64_t at = static_cast<int64_t>(h) * p.lam_stride;
+        const float lam = p.lam_dtype == ELSA_F32 ? static_cast<const float*>(p.lam)[at] : p.lam_dtype == ELSA_F16 ? to_f32(static_cast<const __half*>(p.lam)[at])
+                                                                                                              : to_f32(static_cast<const __nv_bfloat16*>(p.lam)[at]);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int col = VEC == 4 ? lane * 4 + e : lane + 32 * e;
+          if (p.out2 && col < p.v_dim) static_cast<T*>(p.out2)[ro * p.v_dim + col] = from_f32<T>(acc[e]);
+          total[e] -= lam * acc[e];
+        }
+      }
+    }
   }
   T* dst = static_cast<T*>(p.out) + b * p.os.b + h * p.os.h + t * p.os.r;
 #pragma unroll

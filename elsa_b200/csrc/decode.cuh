@@ -31,6 +31,9 @@ struct DecodeParams {
   // the merge
   const void* lam; int lam_dtype, lam_stride;   // maps == 2: out = s1 / z1 - lam[h] s2 / z2, a value for each head or for all (lam_stride 0)
   void* out; Strides os;                // [batch, heads, nq, v_dim]
+  // maps == 2, for a backward (null: not wanted): s2 / z2 as contiguous [batch, heads, nq, v_dim], log2 of each row's sum of 2^score as
+  // [map][batch * heads * nq] (-inf: no key)
+  void* out2; float* lse;
 };
 
 __host__ __device__ inline int64_t decode_rows(const DecodeParams& p) { return static_cast<int64_t>(p.batch) * (p.heads / p.kv_heads) * p.nq; }

@@ -38,6 +38,13 @@ def _check_lengths(lengths, batch, device):
         raise ValueError("lengths must be a contiguous int32 vector [B] on the device of q")
 
 
+def _positive_scale(scale, dim):
+    scale = max(1, int(dim)) ** -0.5 if scale is None else float(scale)
+    if not 0.0 < scale < float("inf"):
+        raise ValueError("scale must be positive and finite")
+    return scale
+
+
 def shared_prefix_attention(
     q: torch.Tensor,
     k_prefix: torch.Tensor,
@@ -79,6 +86,7 @@ def shared_prefix_attention(
     if dim > 128:
         raise ValueError("head_dim > 128 is not supported by the current kernels")
     _check_lengths(lengths, batch, q.device)
+    scale = _positive_scale(scale, dim)
     if q.numel() == 0:
         return torch.empty_like(q)
     n_prefix, n_own = int(k_prefix.shape[1]), int(k.shape[2])
@@ -95,6 +103,6 @@ def shared_prefix_attention(
         rc = _lib.load().elsa_shared_prefix_attention(
             q.data_ptr(), k_prefix.data_ptr(), v_prefix.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), flat,
             None if lengths is None else lengths.data_ptr(), ws.data_ptr(), ws.numel(), dt, batch, heads, kv_heads, nq, dim,
-            n_prefix, n_own, dim ** -0.5 if scale is None else float(scale), _lib.raw_stream(q.device))
+            n_prefix, n_own, scale, _lib.raw_stream(q.device))
     _lib.check(rc, "elsa_shared_prefix_attention")
     return out

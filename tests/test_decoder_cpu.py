@@ -116,3 +116,36 @@ def test_shared_prefix_splits_cover_every_key(lib):
         rows = batch * heads // kv * nq
         least = 2 * kv * rows * (d + 2) * 4
         assert lib.elsa_shared_prefix_workspace_bytes(2, batch, heads, kv, nq, d, p, s) >= least
+
+
+# ---- differential attention -----------------------------------------------------------------------------------------
+def test_differential_lambda():
+    a = [torch.randn(3, 8, generator=torch.Generator().manual_seed(i)) for i in range(4)]
+    got = E.differential_lambda(*a, 0.3)
+    want = torch.exp((a[0] * a[1]).sum(-1)) - torch.exp((a[2] * a[3]).sum(-1)) + 0.3
+    assert torch.allclose(got, want) and got.dtype == torch.float32
+    assert E.differential_lambda(*(x.bfloat16() for x in a), 0.3).dtype == torch.float32
+
+
+def test_differential_refuses_before_any_launch(lib):
+    import ctypes
+    q, k, v = torch.zeros(1, 4, 3, 16), torch.zeros(1, 4, 5, 16), torch.zeros(1, 2, 5, 32)
+    with pytest.raises(ValueError, match="CUDA"):
+        E.differential_attention(q, k, v, 0.5)
+    with pytest.raises(ValueError, match="two heads"):
+        E.differential_attention(q[:, :3], k, v, 0.5)
+    size = lib.elsa_differential_workspace_bytes
+    assert size(1, 1, 4, 2, 3, 100, 64, 128) > 0 and size(1, 1, 4, 2, 3, 0, 64, 128) == 0
+    for bad in ((9, 1, 4, 2, 3, 100, 64, 128), (1, 1, 4, 3, 3, 100, 64, 128), (1, 1, 4, 2, 0, 100, 64, 128), (1, 1, 4, 2, 3, 100, 129, 128),
+                (1, 1, 4, 2, 3, 100, 64, 129), (1, 1, 4, 2, 3, -1, 64, 128), (1, 70000, 4, 2, 3, 100, 64, 128)):
+        assert size(*bad) == -1
+    st = (ctypes.c_int64 * 12)(*([64] * 12))
+
+    def call(q=256, k=256, v=256, lam=256, lam_dtype=0, out=256, strides=st, ws=256, nbytes=1 << 40, dtype=1, heads=4, kv=2, scale=0.125):
+        return lib.elsa_differential_forward(q, k, v, lam, lam_dtype, 0, None, out, strides, None, None, ws, nbytes, dtype, 1, heads, kv, 3, 100,
+                                             64, 128, 0, scale, None)
+
+    for name in ("q", "k", "v", "lam", "out", "strides"):
+        assert call(**{name: None}) == 1
+    assert call(lam_dtype=7) == 1 and call(dtype=7) == 1 and call(kv=3) == 1 and call(scale=0.0) == 1 and call(scale=float("nan")) == 1
+    assert call(ws=None) == 4 and call(ws=100) == 4 and call(nbytes=100) == 4
