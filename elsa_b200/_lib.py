@@ -66,6 +66,8 @@ SIGNATURES = {
     "elsa_shared_prefix_attention": (c_int, [_P] * 9 + [c_int64] + [c_int] * 8 + [c_double, _P]),
     "elsa_differential_workspace_bytes": (c_int64, [c_int] * 8),
     "elsa_differential_forward": (c_int, [_P] * 4 + [c_int, c_int] + [_P] * 6 + [c_int64] + [c_int] * 9 + [c_double, _P]),
+    "elsa_differential_backward_workspace_bytes": (c_int64, [c_int] * 8),
+    "elsa_differential_backward": (c_int, [_P] * 4 + [c_int, c_int] + [_P] * 10 + [c_int64] + [c_int] * 9 + [c_double, _P]),
     "elsa_rotary": (c_int, [_P, _P, _P, c_int, _P, _P, _P, c_int, _P, _P, c_int, c_int64, c_int64, c_double] + [c_int] * 7 + [_P]),
 }
 

@@ -11,7 +11,7 @@ from typing import Optional, Union
 import torch
 
 from . import _lib
-from .attention import _DeviceScope, _cached_bytes
+from .attention import _DeviceScope, _cached_bytes, _in_place_or_copy
 from .shared_prefix import _check_lengths, _positive_scale, _readable, _strides
 
 
@@ -114,3 +114,65 @@ def differential_attention(
     if sizes[0] * sizes[1] * sizes[3] * sizes[6] == 0:
         return torch.empty((sizes[0], sizes[1], sizes[3], sizes[6]), device=q.device, dtype=q.dtype)
     return _forward(q, k, v, lam, sizes, is_causal, scale, lengths, False)[0]
+
+
+def _for_tiles(t):
+    """As the tensor-core kernels read it, in place or copied; other types and head dims as they are."""
+    return _in_place_or_copy(t)[0] if t.dtype != torch.float32 and t.shape[-1] % 8 == 0 and t.numel() else t
+
+
+class _DifferentialAutograd(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, v, lam, sizes, is_causal, scale):
+        out, out2, lse, q, k, v = _forward(_for_tiles(q), _for_tiles(k), _for_tiles(v), lam, sizes, is_causal, scale, None, True)
+        ctx.lam = None if isinstance(lam, torch.Tensor) else lam
+        ctx.save_for_backward(q, k, v, out, out2, lse, *((lam,) if isinstance(lam, torch.Tensor) else ()))
+        ctx.sizes, ctx.is_causal, ctx.scale = sizes, is_causal, scale
+        return out
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dout):
+        q, k, v, out, out2, lse, *rest = ctx.saved_tensors
+        lam = rest[0] if rest else ctx.lam
+        batch, heads, kv_heads, nq, nk, dim, v_dim = ctx.sizes
+        dout, gs = _readable(_for_tiles(dout.to(q.dtype)))
+        dq, dk, dv = (torch.empty(t.shape, device=t.device, dtype=t.dtype) for t in (q, k, v))
+        dlam = torch.empty_like(lam, memory_format=torch.contiguous_format) if rest and ctx.needs_input_grad[3] else None
+        keep, lam_ptr, lam_dtype, lam_stride = _lam_args(lam, heads, q)
+        wide = lam_stride == 0 and dlam is not None and dlam.numel() > 1    # an expanded value: one sum, shared out by autograd
+        if wide:
+            keep = keep.contiguous()
+            lam_ptr, lam_stride = keep.data_ptr(), 1
+        dt = _lib.dtype_code(q.dtype)
+        need = _cached_bytes("elsa_differential_backward_workspace_bytes", dt, *ctx.sizes)
+        flat = (ctypes.c_int64 * 24)(*_strides(q), *_strides(k), *_strides(v), *_strides(out), *gs, *_strides(dq), *_strides(dk), *_strides(dv))
+        with _DeviceScope(q.device):
+            ws = torch.empty((max(need, 256),), device=q.device, dtype=torch.uint8)
+            rc = _lib.load().elsa_differential_backward(
+                q.data_ptr(), k.data_ptr(), v.data_ptr(), lam_ptr, lam_dtype, lam_stride, out.data_ptr(), out2.data_ptr(), lse.data_ptr(),
+                dout.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), None if dlam is None else dlam.data_ptr(), flat,
+                ws.data_ptr(), ws.numel(), dt, *ctx.sizes, int(ctx.is_causal), ctx.scale, _lib.raw_stream(q.device))
+        _lib.check(rc, "elsa_differential_backward")
+        return dq, dk, dv, dlam, None, None, None
+
+
+def differential_attention_train(
+    q: torch.Tensor,
+    k: torch.Tensor,
+    v: torch.Tensor,
+    lam: Union[torch.Tensor, float],
+    *,
+    is_causal: bool = False,
+    scale: Optional[float] = None,
+) -> torch.Tensor:
+    """Differentiable `differential_attention` (without lengths), in q, k, v and, where it is a tensor, lam: the forward keeps P2 v and each
+    row's log sum, the backward recomputes the maps.  Gradients repeat bit for bit; those of shared key heads and of a shared lam are
+    summed."""
+    sizes = _check(q, k, v, lam, "differential_attention_train")
+    scale = _positive_scale(scale, sizes[5])
+    if any(x == 0 for x in (sizes[0], sizes[1], sizes[3], sizes[4], sizes[6])):
+        # nothing to attend to: zeros that depend on nothing but shapes (and have zero gradients)
+        zero = q.sum() * 0 + k.sum() * 0 + v.sum() * 0
+        return torch.zeros((sizes[0], sizes[1], sizes[3], sizes[6]), device=q.device, dtype=q.dtype) + zero.to(q.dtype)
+    return _DifferentialAutograd.apply(q, k, v, lam, sizes, bool(is_causal), scale)

@@ -385,6 +385,16 @@ int elsa_differential_forward(const void* q, const void* k, const void* v, const
                               int64_t workspace_bytes, int dtype, int batch, int heads, int kv_heads, int nq, int nk, int head_dim,
                               int v_dim, int is_causal, double scale, void* stream);
 
+/* Its gradients, from the forward's out, out2 and lse (made without lengths) and dout: dq, dk, dv, and dlam in lam's layout and type
+ * (one value where lam_stride is 0; NULL: not wanted).  `strides` = element strides {batch, head, row} of q, k, v, out, dout, dq, dk, dv.
+ * No atomics: a call repeats bit for bit.  workspace: elsa_differential_backward_workspace_bytes, 256-byte aligned. */
+int64_t elsa_differential_backward_workspace_bytes(int dtype, int batch, int heads, int kv_heads, int nq, int nk, int head_dim, int v_dim);
+int elsa_differential_backward(const void* q, const void* k, const void* v, const void* lam, int lam_dtype, int lam_stride,
+                               const void* out, const void* out2, const float* lse, const void* dout, void* dq, void* dk, void* dv,
+                               void* dlam, const int64_t* strides, void* workspace, int64_t workspace_bytes, int dtype, int batch,
+                               int heads, int kv_heads, int nq, int nk, int head_dim, int v_dim, int is_causal, double scale,
+                               void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -149,3 +149,23 @@ def test_differential_refuses_before_any_launch(lib):
         assert call(**{name: None}) == 1
     assert call(lam_dtype=7) == 1 and call(dtype=7) == 1 and call(kv=3) == 1 and call(scale=0.0) == 1 and call(scale=float("nan")) == 1
     assert call(ws=None) == 4 and call(ws=100) == 4 and call(nbytes=100) == 4
+
+
+def test_differential_backward_refuses_before_any_launch(lib):
+    import ctypes
+    q, k, v = torch.zeros(1, 4, 3, 16), torch.zeros(1, 4, 5, 16), torch.zeros(1, 2, 5, 32)
+    with pytest.raises(ValueError, match="CUDA"):
+        E.differential_attention_train(q, k, v, 0.5)
+    size = lib.elsa_differential_backward_workspace_bytes
+    assert size(1, 2, 4, 2, 3, 100, 64, 128) == 2 * 4 * 4 * 128 * 4 and size(1, 2, 4, 2, 3, 100, 64, 130) == -1
+    st = (ctypes.c_int64 * 24)(*([64] * 24))
+
+    def call(strides=st, ws=256, nbytes=1 << 40, dtype=1, lam_dtype=0, scale=0.125, **null):
+        ptr = [None if name in null else 256 for name in ("q", "k", "v", "lam")]
+        more = [None if name in null else 256 for name in ("out", "out2", "lse", "dout", "dq", "dk", "dv", "dlam")]
+        return lib.elsa_differential_backward(*ptr, lam_dtype, 1, *more, strides, ws, nbytes, dtype, 2, 4, 2, 3, 100, 64, 128, 0, scale, None)
+
+    for name in ("q", "k", "v", "lam", "out", "out2", "lse", "dout", "dq", "dk", "dv"):
+        assert call(**{name: 0}) == 1
+    assert call(strides=None) == 1 and call(dtype=8) == 1 and call(lam_dtype=8) == 1 and call(scale=-1.0) == 1
+    assert call(ws=None) == 4 and call(ws=64) == 4 and call(nbytes=64) == 4

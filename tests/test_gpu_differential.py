@@ -198,3 +198,221 @@ def test_refusals():
     wide = _inputs(1, 1, 1, 3, 9, 64, 136, torch.float16)
     with pytest.raises(ValueError, match="128"):
         E.differential_attention(*wide)
+
+
+# ---- gradients ---------------------------------------------------------------------------------------------------------
+def _gradients(q, k, v, lam, dout, causal, scale=None):
+    """(gradients, limits) in 64 bits, from the formulas.  The limits, with h the half step of the type (2^-24 for fp32), per map m:
+      P        the weight's own error e (as in the forward)
+      D        g . (P V): the saved output's rounding h, of sum_d |g_d| mass_d (mass = P |V|), and SUMS for P V and the dot
+      G        64 or 128 products: (Dv + 8) 2^-24 of sum |g||v|
+      dS       P (G - D): P e |G - D| + P (err G + err D), then one rounding h of it (16-bit: the second product's operand)
+      products sums of at most `terms` roundings of 2^-24 (a tile's accumulators; the FMA kernels add key after key), each operand's error
+               times the other operand's size; then one rounding h of the result"""
+    b, h, hkv, nq, nk, d = q.shape[0], q.shape[1] // 2, v.shape[1], q.shape[2], k.shape[2], q.shape[3]
+    scale = d ** -0.5 if scale is None else scale
+    u, half = 2.0 ** -24, torch.finfo(q.dtype).eps / 2
+    op = half if q.dtype != torch.float32 else 0.0           # operands of the second products are rounded to 16-bit types only
+    grads = [torch.zeros(t.shape, device=q.device, dtype=torch.float64) for t in (q, k, v)] + [torch.zeros(h, device=q.device, dtype=torch.float64)]
+    limits = [torch.zeros_like(t) for t in grads]
+    terms = (max(nq, nk) + 64) * u
+    for i in range(b):
+        for j in range(h):
+            maps, g, _ = _maps(q, k, lam, causal, None, scale, i, j, hkv)
+            w = float(lam[j]) if isinstance(lam, torch.Tensor) and lam.numel() > 1 else float(lam)
+            go, val = dout[i, j].double(), v[i, g].double()
+            gv, gv_size = go @ val.T, go.abs() @ val.abs().T
+            e_gv = (v.shape[3] + 8) * u * gv_size
+            outs = [m.p @ val for m in maps]
+            mass = [m.p @ val.abs() for m in maps]
+            out_size = mass[0] + abs(w) * mass[1]
+            dd = [(go * o).sum(-1, keepdim=True) for o in outs]
+            # D2 from the saved P2 V; D1 = g . out + lam D2 with the saved out
+            e_o = [(m.e + SUMS + op) * s for m, s in zip(maps, mass)]
+            e_d2 = (go.abs() * (e_o[1] + half * outs[1].abs() * 1.01 + 2.0 ** -25)).sum(-1, keepdim=True) + 140 * u * (go.abs() * mass[1]).sum(-1, keepdim=True)
+            e_out = e_o[0] + abs(w) * e_o[1] + half * (outs[0] - w * outs[1]).abs() * 1.01 + 2.0 ** -25
+            e_d1 = (go.abs() * e_out).sum(-1, keepdim=True) + abs(w) * e_d2 + 280 * u * (go.abs() * out_size).sum(-1, keepdim=True)
+            sign = (1.0, -w)
+            ds, e_ds = [], []
+            for m, mp, dm, e_dm in zip((0, 1), maps, dd, (e_d1, e_d2)):
+                x = mp.p * (gv - dm)
+                ex = mp.p * (e_gv + e_dm + 4 * u * (gv.abs() + dm.abs())) + mp.e * x.abs()
+                ds.append(sign[m] * x)
+                e_ds.append(abs(sign[m]) * (ex + op * (x.abs() + ex) + 2.0 ** -26 * (op > 0)))     # (2^-26: fp16 below its normal range)
+            pc = maps[0].p - w * maps[1].p
+            e_pc = maps[0].p * maps[0].e + abs(w) * maps[1].p * maps[1].e
+            e_pc = e_pc + op * (pc.abs() + e_pc) + 4 * u * (maps[0].p + abs(w) * maps[1].p) + 2.0 ** -26 * (op > 0)
+            for m in (0, 1):
+                qm, km = q[i, 2 * j + m].double(), k[i, 2 * g + m].double()
+                grads[0][i, 2 * j + m] += scale * ds[m] @ km
+                limits[0][i, 2 * j + m] += scale * (e_ds[m] + terms * ds[m].abs()) @ km.abs()
+                grads[1][i, 2 * g + m] += scale * ds[m].T @ qm
+                limits[1][i, 2 * g + m] += scale * (e_ds[m] + (h // hkv) * terms * ds[m].abs()).T @ qm.abs()
+            grads[2][i, g] += pc.T @ go
+            limits[2][i, g] += (e_pc + (h // hkv) * terms * pc.abs()).T @ go.abs()
+            grads[3][j] -= dd[1].sum()
+            limits[3][j] += e_d2.sum() + (b * nq + 64) * u * dd[1].abs().sum()
+    for t, lim in zip(grads, limits):
+        lim += half * t.abs() * 1.01 + 2.0 ** -25
+    return grads, limits
+
+
+def _run_train(q, k, v, lam, dout, **kw):
+    leaves = [t.detach().clone().requires_grad_(True) if isinstance(t, torch.Tensor) else t for t in (q, k, v, lam)]
+    out = E.differential_attention_train(*leaves, **kw)
+    return out.detach(), torch.autograd.grad(out, [t for t in leaves if isinstance(t, torch.Tensor)], dout)
+
+
+def _check_gradients(got, q, k, v, lam, dout, causal=False, scale=None):
+    grads, limits = _gradients(q, k, v, lam, dout, causal, scale)
+    names = ("dq", "dk", "dv", "dlam")
+    if len(got) == 4 and got[3].numel() == 1 and grads[3].numel() > 1:
+        grads[3], limits[3] = grads[3].sum().view(got[3].shape), limits[3].sum().view(got[3].shape)
+        if got[3].dtype != q.dtype:
+            limits[3] = limits[3] + torch.finfo(got[3].dtype).eps * grads[3].abs()
+    for name, a, b, lim in zip(names, got, grads, limits):
+        if name == "dlam":
+            lim = lim + torch.finfo(a.dtype).eps / 2 * b.abs() * 1.01
+        err = (a.double() - b.view(a.shape)).abs()
+        assert bool((err <= lim.view(a.shape)).all()), f"{name}: {float((err / lim.view(a.shape)).max())} of the limit"
+    assert _lib.load().elsa_device_status(0) == 0
+
+
+TRAIN = [
+    # b, h, hkv, nq, nk, d, dv
+    (1, 1, 1, 1, 1, 64, 128), (2, 2, 1, 5, 9, 32, 64), (1, 2, 2, 65, 65, 64, 128), (2, 4, 4, 128, 128, 64, 128), (1, 4, 1, 129, 300, 64, 128),
+    (1, 2, 2, 257, 257, 32, 64), (1, 3, 3, 200, 500, 48, 96), (2, 2, 2, 300, 90, 64, 128), (1, 1, 1, 320, 640, 8, 16), (1, 2, 1, 70, 513, 64, 64),
+    (1, 2, 2, 100, 260, 64, 72), (1, 2, 2, 33, 70, 128, 128), (2, 2, 1, 90, 33, 20, 12), (1, 1, 1, 66, 40, 7, 5),
+]
+
+
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("case", TRAIN, ids=str)
+def test_gradients(case, dtype, causal):
+    q, k, v, lam = _inputs(*case, dtype)
+    dout = _normal((case[0], case[1], case[3], case[6]), dtype, 20)
+    out, got = _run_train(q, k, v, lam, dout, is_causal=causal)
+    _check_forward(out, q, k, v, lam, causal=causal)
+    _check_gradients(got, q, k, v, lam, dout, causal)
+    again = _run_train(q, k, v, lam, dout, is_causal=causal)[1]
+    assert all(torch.equal(x, y) for x, y in zip(got, again))
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_gradient_of_lam_in_its_own_type_and_shape(dtype):
+    q, k, v, lam = _inputs(2, 4, 2, 100, 100, 64, 128, dtype)
+    dout = _normal((2, 4, 100, 128), dtype, 21)
+    for lam in (lam, lam.bfloat16(), torch.tensor(0.4, device="cuda"), torch.tensor([0.4], device="cuda", dtype=torch.float16)):
+        out, got = _run_train(q, k, v, lam, dout)
+        assert got[3].shape == lam.shape and got[3].dtype == lam.dtype
+        _check_gradients(got, q, k, v, lam, dout)
+    out, got = _run_train(q, k, v, 0.4, dout)
+    assert len(got) == 3
+    _check_gradients(got, q, k, v, 0.4, dout)
+    # one value expanded over the heads: its gradient is the sum
+    one = torch.tensor([0.4], device="cuda", requires_grad=True)
+    E.differential_attention_train(q, k, v, one.expand(4)).backward(dout)
+    single = _run_train(q, k, v, one, dout)[1][3]
+    assert abs(float(one.grad) - float(single)) <= 2.0 ** -20 * float(_gradients(q, k, v, one.detach(), dout, False)[0][3].abs().sum()) + 4 * 2.0 ** -24
+
+
+def test_gradients_against_differences():
+    """fp32, along random directions: (f(x + e u) - f(x - e u)) / 2e with e = 2^-6 is off by e^2 / 6 times a third derivative and by the
+    roundings of the two sums, 2^-24 times the 768 summands' size over e."""
+    q, k, v, lam = _inputs(1, 2, 1, 12, 12, 16, 32, torch.float32)
+    dout = _normal((1, 2, 12, 32), torch.float32, 22)
+    got = _run_train(q, k, v, lam, dout, is_causal=True)[1]
+    leaves = [q, k, v, lam]
+    e = 2.0 ** -6
+
+    def f(args):
+        return float((E.differential_attention(*args, is_causal=True).double() * dout.double()).sum())
+
+    def exact(args):                 # the same function in 64 bits, to know the third-order term
+        total = 0.0
+        for j in range(2):
+            maps, g, _ = _maps(args[0], args[1], args[3], True, None, None, 0, j, 1)
+            total += float((dout[0, j].double() * ((maps[0].p - float(args[3][j]) * maps[1].p) @ args[2][0, g].double())).sum())
+        return total
+
+    for n in range(4):
+        u = _normal(leaves[n].shape, torch.float32, 30 + n)
+        step = lambda s: [x + s * u if i == n else x for i, x in enumerate(leaves)]
+        diff = (f(step(e)) - f(step(-e))) / (2 * e)
+        third = abs((exact(step(2 * e)) - exact(step(-2 * e))) / (4 * e) - (exact(step(e)) - exact(step(-e))) / (2 * e))   # = e^2 / 2 f'''
+        rounding = 2 * 2.0 ** -20 * float(dout.abs().sum()) / e / 16
+        assert abs(diff - float((got[n].double() * u.double()).sum())) <= third + rounding
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.float32])
+@pytest.mark.parametrize("layout", ["bnhd", "odd_offset", "strided_d", "expanded_dout", "expanded_kv"])
+def test_strided_training(layout, dtype):
+    q, k, v, lam = _inputs(2, 4, 2, 90, 90, 64, 128, dtype)
+    dout = _normal((2, 4, 90, 128), dtype, 23)
+    if layout == "bnhd":
+        q, k, v, dout = (t.transpose(1, 2).contiguous().transpose(1, 2) for t in (q, k, v, dout))
+    elif layout == "odd_offset":
+        q, k, v, dout = (torch.cat((t.new_zeros(1), t.flatten()))[1:].view(t.shape) for t in (q, k, v, dout))
+    elif layout == "strided_d":
+        q, k, v, dout = (t.repeat_interleave(2, -1)[..., ::2] for t in (q, k, v, dout))
+    elif layout == "expanded_dout":
+        dout = torch.ones((), device="cuda", dtype=dtype).expand(2, 4, 90, 128)
+    leaves = [t.detach().requires_grad_(True) for t in (q, k, v, lam)]
+    args = list(leaves)
+    if layout == "expanded_kv":
+        leaves[1] = k[:1].detach().clone().requires_grad_(True)
+        args[1] = leaves[1].expand_as(k)
+    out = E.differential_attention_train(*args, is_causal=True)
+    got = list(torch.autograd.grad(out, args, dout))
+    _check_gradients(got, *(t.detach() for t in args), dout, causal=True)
+
+
+def test_some_inputs_without_gradients_and_no_keys():
+    q, k, v, lam = _inputs(1, 2, 2, 70, 70, 64, 128, torch.float16)
+    k.requires_grad_(True)
+    out = E.differential_attention_train(q, k, v, lam)
+    out.sum().backward()
+    assert k.grad is not None and q.grad is None and lam.grad is None
+    e = torch.empty((1, 4, 0, 64), device="cuda", dtype=torch.float16, requires_grad=True)
+    q.requires_grad_(True)
+    out = E.differential_attention_train(q, e, v[:, :, :0], lam)
+    out.sum().backward()
+    assert not bool(out.any()) and not bool(q.grad.any()) and e.grad.shape == e.shape
+
+
+def test_a_changed_input_is_noticed():
+    q, k, v, lam = _inputs(1, 1, 1, 70, 70, 64, 128, torch.float16)
+    q.requires_grad_(True)
+    out = E.differential_attention_train(q, k, v, lam)
+    k.mul_(2)
+    with pytest.raises(RuntimeError, match="modified by an inplace"):
+        out.sum().backward()
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_training_step_on_another_stream_and_captured(dtype):
+    q, k, v, lam = (t.requires_grad_(True) for t in _inputs(1, 4, 2, 200, 200, 64, 128, dtype))
+    dout = _normal((1, 4, 200, 128), dtype, 24)
+
+    def step():
+        out = E.differential_attention_train(q, k, v, lam, is_causal=True)
+        return (out,) + torch.autograd.grad(out, (q, k, v, lam), dout)
+
+    want = [t.detach().clone() for t in step()]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got = step()
+    torch.cuda.current_stream().wait_stream(side)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    del got
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        held = step()
+    with torch.no_grad():
+        q.copy_(q.flip(2).clone())
+    graph.replay()
+    torch.cuda.synchronize()
+    fresh = step()
+    assert all(torch.equal(a, b) for a, b in zip(held, fresh))
