@@ -272,5 +272,5 @@ extern "C" int elsa_differential_backward(const void* q, const void* k, const vo
                      (nk == 0 || (diff_rows_ok(dk, d.dks, head_dim, 2 * kv_heads, batch) && diff_rows_ok(dv, d.dvs, v_dim, kv_heads, batch)));
   if (tiles && (rc = device_status_ok()) != ELSA_OK) return rc;
   if ((rc = diff_stats(d, stats, dtype, st)) != ELSA_OK) return rc;
-  return tiles ? diff_bwd_tc(d, stats, dtype, st) : diff_bwd_simt(d, stats, dtype, st);
+  return tiles ? diff_bwd_tc(d, stats, dtype, st) : diff_bwd_any(d, stats, dtype, st);
 }

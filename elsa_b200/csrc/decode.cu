@@ -1,5 +1,5 @@
 // Few query rows over long key caches: each CTA folds one range of keys of one kv head into the (m, z, s) summaries of up to
-// 16 (tensor cores) or 32 (FMA) rows -- all query heads that share the kv head, and all query tokens, are rows of one tile, so
+// 16 (16-bit types) or 32 (any type) rows -- all query heads that share the kv head, and all query tokens, are rows of one tile, so
 // a cache is read once -- and a second launch merges a row's summaries.
 //
 // Bound: the bytes of the caches; rows are few, so the products are small.
@@ -9,7 +9,7 @@
 //                      with running max, sum and O in registers; the four are merged through shared memory at the end.  mma.sync
 //                      and not tcgen05: a tile has 16 rows here and not 128, a warp's products stay in its registers, and 8
 //                      bytes are loaded for every row's multiply-add that either could do.
-//   split_simt_kernel  any type, any head dim up to 128, any stride: FP32 FMAs on 32 x 32 tiles.
+//   split_any_kernel   any type, any head dim up to 128, any stride, in fp32 (split tf32 operands) on 32 x 32 tiles.
 //   merge_kernel       a warp per row.
 //
 // Softmax statistics, sums and O are fp32; P is rounded to the inputs' type for the second product (its error, half a step of
@@ -19,13 +19,14 @@
 
 #include "decode.cuh"
 #include "tc_common.cuh"
+#include "tf32.cuh"
 
 namespace elsa {
 
 namespace {
 
 constexpr int kMmaWarps = 4, kMmaThreads = 32 * kMmaWarps, kMmaRows = 16, kMmaKeys = 16, kStages = 3;
-constexpr int kSimtThreads = 128, kSimtRows = 32, kSimtKeys = 32, kSimtDim = 128;
+constexpr int kAnyThreads = 128, kAnyRows = 32, kAnyKeys = 32, kAnyDim = 128;
 constexpr float kRescaleThreshold = 8.f;
 
 struct Block { int seg, g, b, row0, n_rows, k0, k1, part, len; };   // rows row0 .. row0 + n_rows of kv head g, keys k0 .. k1
@@ -290,129 +291,154 @@ split_mma_kernel(const DecodeParams p) {
   }
 }
 
-// ---- FMA --------------------------------------------------------------------------------------------------------------
-// 32 rows x 32 keys; a thread has rows (t / 8) * 2 + {0, 1} and keys t % 8 + 8 {0..3} of the scores, then the same rows and
-// value columns (t % 8) * 4 + 32 {0..3} of O.  Shared rows are 4 floats longer than their columns (no bank is met twice by the
-// eight threads of a row).
+// ---- any type ---------------------------------------------------------------------------------------------------------
+// 32 rows x 32 keys in fp32, products on split tf32 operands (tf32.cuh).  Four warps: 16 rows each, and of two maps one, or of one
+// map's keys the first or the second 16 (whose summaries are merged at the end).  A warp's weights go from its score accumulators
+// straight into the second product.
 template <typename T, int MAPS>
-__global__ void __launch_bounds__(kSimtThreads)
-split_simt_kernel(const DecodeParams p) {
+__global__ void __launch_bounds__(kAnyThreads)
+split_any_kernel(const DecodeParams p) {
   extern __shared__ __align__(16) float fsmem[];
-  constexpr int kPitch = kSimtDim + 4, kScorePitch = kSimtKeys + 1;
+  constexpr int kPitch = kAnyDim + 4, kBlocks = MAPS == 2 ? 4 : 2;     // 8-key blocks of a warp's scores
   float* sq = fsmem;                                    // [map][row][dim]
-  float* sk = sq + MAPS * kSimtRows * kPitch;           // [map][key][dim]
-  float* sv = sk + MAPS * kSimtKeys * kPitch;           // [key][dim]
-  float* sp = sv + kSimtKeys * kPitch;                  // [map][row][key]
+  float* sk = sq + MAPS * kAnyRows * kPitch;            // [map][key][dim]
+  float* sv = sk + MAPS * kAnyKeys * kPitch;            // [key][dim]
   Block w;
-  if (!locate(p, kSimtRows, w)) return;
+  if (!locate(p, kAnyRows, w)) return;
   const DecodeSegment& sg = p.seg[w.seg];
-  const int tid = threadIdx.x, r0 = tid / 8 * 2, kc = tid % 8;
-  const int dim4 = (p.head_dim + 3) / 4 * 4;
-  for (int i = tid; i < MAPS * kSimtRows * dim4; i += kSimtThreads) {
-    const int col = i % dim4, rm = i / dim4, r = rm % kSimtRows, m = rm / kSimtRows;
-    const bool real = r < w.n_rows && col < p.head_dim;
-    sq[(m * kSimtRows + r) * kPitch + col] = real ? to_f32<T>(static_cast<const T*>(p.q)[q_offset(p, w.g, w.row0 + r, m) + col]) : 0.f;
-  }
-  int lim[2];
-#pragma unroll
-  for (int j = 0; j < 2; ++j) lim[j] = r0 + j < w.n_rows ? min(w.k1, row_limit(p, sg, w.len, w.row0 + r0 + j)) : 0;
-  float m_run[MAPS][2], z[MAPS][2], o[MAPS][2][16];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, half = warp & 1, map = MAPS == 2 ? warp >> 1 : 0, part = MAPS == 2 ? 0 : warp >> 1;
+  const int d8 = (p.head_dim + 7) / 8 * 8, v8 = (p.v_dim + 7) / 8 * 8;
+  const int kc = threadIdx.x % 8;
+  // (query rows are not evenly spaced: row by row)
 #pragma unroll
   for (int m = 0; m < MAPS; ++m)
+    for (int r = threadIdx.x / 8; r < kAnyRows; r += kAnyThreads / 8) {
+      const bool real = r < w.n_rows;
+      const T* src = static_cast<const T*>(p.q) + (real ? q_offset(p, w.g, w.row0 + r, m) : 0);
+      for (int col = kc; col < kAnyDim; col += 8) sq[(m * kAnyRows + r) * kPitch + col] = real && col < p.head_dim ? to_f32<T>(src[col]) : 0.f;
+    }
+  using KeyRows = tf32::Rows<T, kAnyThreads, kAnyKeys, kAnyDim>;
+  const int64_t k_base = (sg.shared ? 0 : w.b * sg.ks.b) + static_cast<int64_t>(MAPS * w.g) * sg.ks.h;
+  const KeyRows k1(sg.k, k_base, sg.ks.r, w.k1, p.head_dim), k2(sg.k, k_base + (MAPS - 1) * sg.ks.h, sg.ks.r, w.k1, p.head_dim);
+  const KeyRows vr(sg.v, (sg.shared ? 0 : w.b * sg.vs.b) + static_cast<int64_t>(w.g) * sg.vs.h, sg.vs.r, w.k1, p.v_dim);
+  const int row = 16 * half + (lane >> 2);              // and row + 8
+  int lim[2];
+  float m_run[2] = {-CUDART_INF_F, -CUDART_INF_F}, z[2] = {0.f, 0.f}, o[kAnyDim / 8][4] = {};
+#pragma unroll
+  for (int j = 0; j < 2; ++j) lim[j] = row + 8 * j < w.n_rows ? min(w.k1, row_limit(p, sg, w.len, w.row0 + row + 8 * j)) : 0;
+  for (int key0 = w.k0; key0 < w.k1; key0 += kAnyKeys) {
+    __syncthreads();
+    k1.load(sk, kPitch, key0);
+    if (MAPS == 2) k2.load(sk + kAnyKeys * kPitch, kPitch, key0);
+    vr.load(sv, kPitch, key0);
+    __syncthreads();
+    float s[kBlocks][4] = {};
+    const float* a = sq + (map * kAnyRows + 16 * half) * kPitch;
+    const float* b = sk + (map * kAnyKeys + 16 * part) * kPitch;
+#pragma unroll 2
+    for (int k = 0; k < d8; k += 8) {
+      tf32::Split x[4], y[2];
+      tf32::load_a(x, a + k, kPitch, lane);
+#pragma unroll
+      for (int n = 0; n < kBlocks; ++n) {
+        tf32::load_bt(y, b + 8 * n * kPitch + k, kPitch, lane);
+        tf32::mma3(s[n], x, y);
+      }
+    }
+    const int key = key0 + 16 * part + 2 * (lane & 3);
+    float top[2] = {-CUDART_INF_F, -CUDART_INF_F}, alpha[2];
+#pragma unroll
+    for (int n = 0; n < kBlocks; ++n)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        s[n][e] = key + 8 * n + (e & 1) < lim[e >> 1] ? s[n][e] * p.scale_log2 : -CUDART_INF_F;
+        top[e >> 1] = fmaxf(top[e >> 1], s[n][e]);
+      }
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
-      m_run[m][j] = -CUDART_INF_F; z[m][j] = 0.f;
-#pragma unroll
-      for (int e = 0; e < 16; ++e) o[m][j][e] = 0.f;
+      top[j] = fmaxf(top[j], __shfl_xor_sync(0xffffffffu, top[j], 1));
+      top[j] = fmaxf(top[j], __shfl_xor_sync(0xffffffffu, top[j], 2));
+      const float m_new = fmaxf(m_run[j], top[j]);
+      alpha[j] = m_new > m_run[j] ? exp2f(m_run[j] - m_new) : 1.f;
+      m_run[j] = m_new;
+      z[j] *= alpha[j];
     }
-  const T* vp = static_cast<const T*>(sg.v) + (sg.shared ? 0 : w.b * sg.vs.b) + static_cast<int64_t>(w.g) * sg.vs.h;
-  for (int key0 = w.k0; key0 < w.k1; key0 += kSimtKeys) {
-    __syncthreads();
-    for (int i = tid; i < MAPS * kSimtKeys * dim4; i += kSimtThreads) {
-      const int col = i % dim4, km = i / dim4, j = km % kSimtKeys, m = km / kSimtKeys;
-      const T* kp = static_cast<const T*>(sg.k) + (sg.shared ? 0 : w.b * sg.ks.b) + static_cast<int64_t>(MAPS * w.g + m) * sg.ks.h;
-      sk[(m * kSimtKeys + j) * kPitch + col] = key0 + j < w.k1 && col < p.head_dim ? to_f32<T>(kp[static_cast<int64_t>(key0 + j) * sg.ks.r + col]) : 0.f;
+    if (__any_sync(0xffffffffu, alpha[0] != 1.f || alpha[1] != 1.f)) {
+#pragma unroll
+      for (int n = 0; n < kAnyDim / 8; ++n)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[n][e] *= alpha[e >> 1];
     }
-    for (int i = tid; i < kSimtKeys * kSimtDim; i += kSimtThreads) {
-      const int col = i % kSimtDim, j = i / kSimtDim;
-      sv[j * kPitch + col] = key0 + j < w.k1 && col < p.v_dim ? to_f32<T>(vp[static_cast<int64_t>(key0 + j) * sg.vs.r + col]) : 0.f;
-    }
-    __syncthreads();
 #pragma unroll
-    for (int m = 0; m < MAPS; ++m) {
-      float s[2][4] = {};
-      for (int d = 0; d < dim4; d += 4) {
-        float4 a[2], b[4];
+    for (int n = 0; n < kBlocks; ++n)
 #pragma unroll
-        for (int j = 0; j < 2; ++j) a[j] = *reinterpret_cast<const float4*>(sq + (m * kSimtRows + r0 + j) * kPitch + d);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) b[e] = *reinterpret_cast<const float4*>(sk + (m * kSimtKeys + kc + 8 * e) * kPitch + d);
-#pragma unroll
-        for (int j = 0; j < 2; ++j)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) s[j][e] = fmaf(a[j].x, b[e].x, fmaf(a[j].y, b[e].y, fmaf(a[j].z, b[e].z, fmaf(a[j].w, b[e].w, s[j][e]))));
+      for (int e = 0; e < 4; ++e) {
+        s[n][e] = exp2f(s[n][e] - (m_run[e >> 1] == -CUDART_INF_F ? 0.f : m_run[e >> 1]));
+        z[e >> 1] += s[n][e];
       }
+#pragma unroll
+    for (int k = 0; k < kBlocks; ++k) {
+      tf32::Split x[4], y[2];
+      tf32::acc_as_a(x, s[k]);
+#pragma unroll
+      for (int n = 0; n < kAnyDim / 8; ++n) {
+        if (8 * n >= v8) continue;
+        tf32::load_b(y, sv + (16 * part + 8 * k) * kPitch + 8 * n, kPitch, lane);
+        tf32::mma3(o[n], x, y);
+      }
+    }
+  }
+#pragma unroll
+  for (int j = 0; j < 2; ++j) {
+    z[j] += __shfl_xor_sync(0xffffffffu, z[j], 1);
+    z[j] += __shfl_xor_sync(0xffffffffu, z[j], 2);
+  }
+  if (MAPS == 1) {                                      // the second 16 keys' summaries through shared memory (over the rows of Q)
+    __syncthreads();
+    float* buffer = fsmem;
+    const int c = 2 * (lane & 3);
+    if (part == 1) {
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
-        float top = -CUDART_INF_F;
+        float* dst = buffer + (row + 8 * j) * kPitch;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          s[j][e] = key0 + kc + 8 * e < lim[j] ? s[j][e] * p.scale_log2 : -CUDART_INF_F;
-          top = fmaxf(top, s[j][e]);
-        }
-#pragma unroll
-        for (int x = 1; x < 8; x <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
-        const float m_new = fmaxf(m_run[m][j], top), m_use = m_new == -CUDART_INF_F ? 0.f : m_new;
-        const float alpha = m_new == -CUDART_INF_F ? 1.f : exp2f(m_run[m][j] - m_new);
-        m_run[m][j] = m_new;
-        z[m][j] *= alpha;
-#pragma unroll
-        for (int e = 0; e < 16; ++e) o[m][j][e] *= alpha;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const float x = exp2f(s[j][e] - m_use);
-          z[m][j] += x;
-          sp[(m * kSimtRows + r0 + j) * kScorePitch + kc + 8 * e] = x;
-        }
+        for (int n = 0; n < kAnyDim / 8; ++n) { dst[8 * n + c] = o[n][2 * j]; dst[8 * n + c + 1] = o[n][2 * j + 1]; }
+        if ((lane & 3) == 0) { dst[kAnyDim] = m_run[j]; dst[kAnyDim + 1] = z[j]; }
       }
     }
-    __syncwarp();                                       // a row's weights come from eight lanes of one warp
-    for (int j = 0; j < kSimtKeys; ++j) {
-      float4 b[4];
+    __syncthreads();
+    if (part == 1) return;                              // (no barrier follows)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) b[e] = *reinterpret_cast<const float4*>(sv + j * kPitch + kc * 4 + 32 * e);
+    for (int j = 0; j < 2; ++j) {
+      const float* src = buffer + (row + 8 * j) * kPitch;
+      const float m2 = src[kAnyDim], z2 = src[kAnyDim + 1], m_new = fmaxf(m_run[j], m2);
+      const float f1 = z[j] != 0.f ? exp2f(m_run[j] - m_new) : 0.f, f2 = z2 != 0.f ? exp2f(m2 - m_new) : 0.f;
+      z[j] = z[j] * f1 + z2 * f2;
+      m_run[j] = m_new;
 #pragma unroll
-      for (int m = 0; m < MAPS; ++m)
-#pragma unroll
-        for (int r = 0; r < 2; ++r) {
-          const float x = sp[(m * kSimtRows + r0 + r) * kScorePitch + j];
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            o[m][r][4 * e] = fmaf(x, b[e].x, o[m][r][4 * e]); o[m][r][4 * e + 1] = fmaf(x, b[e].y, o[m][r][4 * e + 1]);
-            o[m][r][4 * e + 2] = fmaf(x, b[e].z, o[m][r][4 * e + 2]); o[m][r][4 * e + 3] = fmaf(x, b[e].w, o[m][r][4 * e + 3]);
-          }
-        }
+      for (int n = 0; n < kAnyDim / 8; ++n) {
+        o[n][2 * j] = o[n][2 * j] * f1 + src[8 * n + c] * f2;
+        o[n][2 * j + 1] = o[n][2 * j + 1] * f1 + src[8 * n + c + 1] * f2;
+      }
     }
   }
   const int64_t base = (static_cast<int64_t>(w.part) * p.kv_heads + w.g) * decode_rows(p) + w.row0;
 #pragma unroll
-  for (int m = 0; m < MAPS; ++m)
+  for (int j = 0; j < 2; ++j) {
+    if (row + 8 * j >= w.n_rows) continue;
+    const int64_t at = (base + row + 8 * j) * MAPS + map;
 #pragma unroll
-    for (int j = 0; j < 2; ++j) {
+    for (int n = 0; n < kAnyDim / 8; ++n)
 #pragma unroll
-      for (int x = 1; x < 8; x <<= 1) z[m][j] += __shfl_xor_sync(0xffffffffu, z[m][j], x);
-      if (r0 + j >= w.n_rows) continue;
-      const int64_t at = (base + r0 + j) * MAPS + m;
-#pragma unroll
-      for (int e = 0; e < 16; ++e) {
-        const int col = kc * 4 + 32 * (e / 4) + e % 4;
-        if (col < p.v_dim) p.s[at * p.v_dim + col] = o[m][j][e];
+      for (int e = 0; e < 2; ++e) {
+        const int col = 8 * n + 2 * (lane & 3) + e;
+        if (col < p.v_dim) p.s[at * p.v_dim + col] = o[n][2 * j + e];
       }
-      if (kc == 0) {
-        p.m[at] = z[m][j] != 0.f ? m_run[m][j] : -CUDART_INF_F;
-        p.z[at] = z[m][j];
-      }
+    if ((lane & 3) == 0) {
+      p.m[at] = z[j] != 0.f ? m_run[j] : -CUDART_INF_F;
+      p.z[at] = z[j];
     }
+  }
 }
 
 // ---- merge ------------------------------------------------------------------------------------------------------------
@@ -555,12 +581,12 @@ int launch_mma_t(const DecodeParams& p, int64_t blocks, cudaStream_t st) {
 }
 
 template <typename T>
-int launch_simt_t(const DecodeParams& p, int64_t blocks, cudaStream_t st) {
-  const auto kernel = p.maps == 2 ? &split_simt_kernel<T, 2> : &split_simt_kernel<T, 1>;
-  const int smem = 4 * ((p.maps * (kSimtRows + kSimtKeys) + kSimtKeys) * (kSimtDim + 4) + p.maps * kSimtRows * (kSimtKeys + 1));
+int launch_any_t(const DecodeParams& p, int64_t blocks, cudaStream_t st) {
+  const auto kernel = p.maps == 2 ? &split_any_kernel<T, 2> : &split_any_kernel<T, 1>;
+  const int smem = 4 * (p.maps * (kAnyRows + kAnyKeys) + kAnyKeys) * (kAnyDim + 4);
   const int rc = ensure_dynamic_smem(reinterpret_cast<const void*>(kernel), smem);
   if (rc != ELSA_OK) return rc;
-  kernel<<<static_cast<unsigned>(blocks), kSimtThreads, smem, st>>>(p);
+  kernel<<<static_cast<unsigned>(blocks), kAnyThreads, smem, st>>>(p);
   ELSA_LAUNCH_CHECK();
   return ELSA_OK;
 }
@@ -581,9 +607,9 @@ bool decode_mma_ok(const DecodeParams& p, int dtype) {
 }
 
 int decode_split(DecodeParams& p, int dtype, cudaStream_t st) {
-  if (p.head_dim > kSimtDim || p.v_dim > kSimtDim) return ELSA_ERR_UNSUPPORTED;
+  if (p.head_dim > kAnyDim || p.v_dim > kAnyDim) return ELSA_ERR_UNSUPPORTED;
   const bool mma = decode_mma_ok(p, dtype);
-  const int tile = mma ? kMmaRows : kSimtRows;
+  const int tile = mma ? kMmaRows : kAnyRows;
   const int rows_b = p.heads / p.kv_heads * p.nq;
   int64_t blocks = 0;
   for (int i = 0; i < p.n_segs; ++i) {
@@ -595,8 +621,8 @@ int decode_split(DecodeParams& p, int dtype, cudaStream_t st) {
   if (blocks == 0) return ELSA_OK;
   if (blocks > 0x7fffffffll) return ELSA_ERR_UNSUPPORTED;
   if (mma) return dtype == ELSA_F16 ? launch_mma_t<__half>(p, blocks, st) : launch_mma_t<__nv_bfloat16>(p, blocks, st);
-  if (dtype == ELSA_F32) return launch_simt_t<float>(p, blocks, st);
-  return dtype == ELSA_F16 ? launch_simt_t<__half>(p, blocks, st) : launch_simt_t<__nv_bfloat16>(p, blocks, st);
+  if (dtype == ELSA_F32) return launch_any_t<float>(p, blocks, st);
+  return dtype == ELSA_F16 ? launch_any_t<__half>(p, blocks, st) : launch_any_t<__nv_bfloat16>(p, blocks, st);
 }
 
 int decode_pack_q(const DecodeParams& p, void* packed, cudaStream_t st) {

@@ -26,11 +26,11 @@ struct DiffParams {
 bool diff_tc_sizes(int dtype, int head_dim, int v_dim);
 bool diff_rows_ok(const void* base, const Strides& s, int row, int heads, int batch);
 int diff_tc_fwd(const DiffParams& p, int dtype, cudaStream_t st);
-// row statistics of the backward, [B * heads][-LSE1, -LSE2, -D1, -D2][n_pad] with n_pad = nq rounded up to 128, and dlam (diff_simt.cu)
+// row statistics of the backward, [B * heads][-LSE1, -LSE2, -D1, -D2][n_pad] with n_pad = nq rounded up to 128, and dlam (diff_any.cu)
 inline int64_t diff_stats_bytes(int batch, int heads, int nq) { return static_cast<int64_t>(batch) * heads * 4 * align_up(nq, 128) * 4; }
 int diff_stats(const DiffParams& p, float* stats, int dtype, cudaStream_t st);
-// dq, dk, dv from them: FP32 FMAs (diff_simt.cu), tensor cores (diff_bwd_tc.cu)
-int diff_bwd_simt(const DiffParams& p, const float* stats, int dtype, cudaStream_t st);
+// dq, dk, dv from them: of any type (diff_any.cu), 16-bit in tiles (diff_bwd_tc.cu)
+int diff_bwd_any(const DiffParams& p, const float* stats, int dtype, cudaStream_t st);
 int diff_bwd_tc(const DiffParams& p, const float* stats, int dtype, cudaStream_t st);
 
 __device__ __forceinline__ float diff_lam(const DiffParams& p, int h) {

@@ -1,5 +1,5 @@
 // Differential attention, backward, on the 5th-generation tensor cores (fp16 / bf16, head dim <= 64, value dim <= 128, multiples of 8).
-// The formulas are in diff_simt.cu.  Nine products for each pair of tiles, G = g V^T shared by the two maps, no atomics:
+// The formulas are in diff_any.cu.  Nine products for each pair of tiles, G = g V^T shared by the two maps, no atomics:
 //
 //   dq body    one CTA per 128 query rows of an output head, 64-key tiles streamed through a 4-stage ring:
 //                S1 = Q1 K1^T, S2 = Q2 K2^T, G = g V^T                                (N = 64)
