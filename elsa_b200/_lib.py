@@ -93,7 +93,9 @@ def load():
 
 _HOST_ENTRIES = ("elsa_forward_workspace_bytes", "elsa_twopass_forward", "elsa_twopass_forward_strided",
                  "elsa_backward_workspace_bytes", "elsa_twopass_backward", "elsa_twopass_backward_strided", "elsa_strerror",
-                 "elsa_last_cuda_error")
+                 "elsa_last_cuda_error", "elsa_rotary", "elsa_shared_prefix_workspace_bytes", "elsa_shared_prefix_attention",
+                 "elsa_differential_workspace_bytes", "elsa_differential_forward", "elsa_differential_backward_workspace_bytes",
+                 "elsa_differential_backward")
 _host_module = None
 _host_tried = False
 

@@ -16,7 +16,8 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 OBJ_DIR = os.path.join(CSRC, "build")
 LIB_PATH = os.path.join(HERE, "libelsa_b200.so")
-HOST_SRC = os.path.join(CSRC, "host.cpp")
+HOST_SRCS = [os.path.join(CSRC, f) for f in ("host.cpp", "host_decoder.cpp")]
+HOST_HEADER = os.path.join(CSRC, "host_common.h")
 HOST_PATH = os.path.join(HERE, "_host.so")
 HOST_STAMP = os.path.join(OBJ_DIR, "_host.built_for")
 SOURCES = ["api.cu", "phase2.cu", "fold_simt.cu", "bwd_simt.cu", "fold_tc.cu", "fold_tc3.cu", "fold_tcw.cu", "bwd_tc.cu", "bwd_tc3.cu", "bwd_tcw.cu", "win_tc.cu", "peaks.cu",
@@ -54,7 +55,7 @@ def _host_built_for() -> str:
 
 
 def host_needs_build() -> bool:
-    newest = max(os.path.getmtime(HOST_SRC), os.path.getmtime(os.path.join(os.path.dirname(HERE), "include", "elsa_b200.h")))
+    newest = max(os.path.getmtime(path) for path in (*HOST_SRCS, HOST_HEADER, os.path.join(os.path.dirname(HERE), "include", "elsa_b200.h")))
     if not os.path.exists(HOST_PATH) or os.path.getmtime(HOST_PATH) < newest or not os.path.exists(HOST_STAMP):
         return True
     with open(HOST_STAMP) as f:
@@ -70,14 +71,24 @@ def build_host() -> None:
     include = [os.path.join(root, "include"), os.path.join(root, "include", "torch", "csrc", "api", "include"),
                sysconfig.get_paths()["include"], os.path.join(cuda, "include")]
     lib = os.path.join(root, "lib")
-    cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden",
-           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", f'-DELSA_TORCH_VERSION="{torch.__version__}"', *(f"-I{path}" for path in include), HOST_SRC,
-           "-o", HOST_PATH, f"-L{lib}", "-ltorch_python", "-ltorch_cuda", "-ltorch_cpu", "-ltorch", "-lc10_cuda", "-lc10",
-           f"-Wl,-rpath,{lib}"]
-    res = subprocess.run(cmd, capture_output=True, text=True)
-    if res.returncode != 0:
-        raise RuntimeError(f"g++ failed for host.cpp:\n{res.stdout}\n{res.stderr}")
+    cxx = os.environ.get("CXX", "g++")
     os.makedirs(OBJ_DIR, exist_ok=True)
+
+    def run(cmd, what):
+        res = subprocess.run(cmd, capture_output=True, text=True)
+        if res.returncode != 0:
+            raise RuntimeError(f"g++ failed for {what}:\n{res.stdout}\n{res.stderr}")
+
+    def compile_one(src: str) -> str:
+        obj = os.path.join(OBJ_DIR, os.path.basename(src).replace(".cpp", ".host.o"))
+        run([cxx, "-O2", "-std=c++17", "-fPIC", "-fvisibility=hidden", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+             f'-DELSA_TORCH_VERSION="{torch.__version__}"', *(f"-I{path}" for path in include), "-c", src, "-o", obj], os.path.basename(src))
+        return obj
+
+    with ThreadPoolExecutor(max_workers=len(HOST_SRCS)) as pool:
+        objs = list(pool.map(compile_one, HOST_SRCS))
+    run([cxx, "-shared", *objs, "-o", HOST_PATH, f"-L{lib}", "-ltorch_python", "-ltorch_cuda", "-ltorch_cpu", "-ltorch", "-lc10_cuda", "-lc10",
+         f"-Wl,-rpath,{lib}"], "_host.so")
     with open(HOST_STAMP, "w") as f:
         f.write(_host_built_for())
 

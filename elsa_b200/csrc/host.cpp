@@ -10,27 +10,11 @@
 // dispatch modes, a wrong shape, dtype or device): the Python operators then take their general path, which also raises
 // the errors.  Layout rules are those of elsa_b200/attention.py: operands are read in place when the D axis is
 // contiguous and rows start on 16-byte boundaries, otherwise copied first; `out` follows q's axis order in memory.
-#define PY_SSIZE_T_CLEAN
-#include <torch/csrc/python_headers.h>
-
-#include <ATen/ATen.h>
-#include <ATen/TracerMode.h>
-#include <ATen/cuda/EmptyTensor.h>
-#include <c10/core/impl/TorchDispatchModeTLS.h>
-#include <c10/cuda/CUDACachingAllocator.h>
-#include <c10/cuda/CUDAGuard.h>
-#include <c10/cuda/CUDAStream.h>
-#include <torch/csrc/Exceptions.h>
-#include <torch/csrc/autograd/function.h>
-#include <torch/csrc/autograd/functions/utils.h>
-#include <torch/csrc/autograd/python_variable.h>
-#include <torch/csrc/autograd/saved_variable.h>
-#include <torch/csrc/dynamo/compiled_autograd.h>
-
-#include "../../include/elsa_b200.h"
+#include "host_common.h"
 
 namespace {
 
+using namespace elsa_host;
 using torch::autograd::SavedVariable;
 using torch::autograd::variable_list;
 
@@ -41,76 +25,15 @@ decltype(&elsa_twopass_forward_strided) f_fwd_strided = nullptr;
 decltype(&elsa_backward_workspace_bytes) f_bwd_ws = nullptr;
 decltype(&elsa_twopass_backward) f_bwd = nullptr;
 decltype(&elsa_twopass_backward_strided) f_bwd_strided = nullptr;
-decltype(&elsa_strerror) f_strerror = nullptr;
-decltype(&elsa_last_cuda_error) f_last_cuda_error = nullptr;
-
-void check_status(int rc, const char* what) {
-  if (rc == ELSA_OK) return;
-  std::string msg = std::string(what) + ": " + f_strerror(rc);
-  if (rc == ELSA_ERR_CUDA) msg += " [cudaError " + std::to_string(f_last_cuda_error()) + "]";
-  if (rc == ELSA_ERR_INVALID_ARGUMENT || rc == ELSA_ERR_UNSUPPORTED) TORCH_CHECK_VALUE(false, msg);
-  throw std::runtime_error(msg);
-}
-
-int dtype_code(at::ScalarType t) {
-  return t == at::kFloat ? ELSA_F32 : t == at::kHalf ? ELSA_F16 : t == at::kBFloat16 ? ELSA_BF16 : -1;
-}
-
 struct Call {                 // the problem, as the C ABI wants it
   int batch, heads, n, d, dt, sdt, causal, part_width, q_chunk;
 };
-
-struct View {                 // a [B, H, N, D] operand: first element and {batch, head, row} element strides
-  char* p = nullptr;
-  int64_t st[3] = {0, 0, 0};
-};
-
-bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
-
-char* data_of(const at::Tensor& t) { return static_cast<char*>(const_cast<void*>(t.const_data_ptr())); }
-
-// fills *v; true when the kernels can read `t` in place
-bool in_place_view(const at::Tensor& t, View* v) {
-  const auto sz = t.sizes();
-  const auto st = t.strides();
-  v->p = data_of(t);
-  for (int i = 0; i < 3; ++i) v->st[i] = sz[i] > 1 ? st[i] : sz[3] * 8;   // (a size-1 axis may have any stride)
-  if ((sz[3] > 1 && st[3] != 1) || !aligned16(v->p)) return false;
-  return ((v->st[0] | v->st[1] | v->st[2]) % 8 == 0) && v->st[0] > 0 && v->st[1] > 0 && v->st[2] >= sz[3];
-}
-
-at::Tensor aligned(const at::Tensor& t) {
-  at::Tensor c = t.contiguous();
-  return aligned16(c.const_data_ptr()) ? c : c.clone();
-}
-
-at::Tensor new_tensor(at::IntArrayRef sizes, const at::Tensor& like, at::ScalarType dtype) {
-  return at::detail::empty_cuda(sizes, dtype, like.device(), std::nullopt);
-}
-
-// an uninitialised [B, H, N, D] tensor in row-major [B, N, H, D] memory
-at::Tensor new_bnhd(const at::Tensor& like, int64_t b, int64_t h, int64_t n, int64_t d) {
-  return at::detail::empty_strided_cuda({b, h, n, d}, {n * h * d, d, h * d, 1}, like.scalar_type(), like.device());
-}
 
 // an uninitialised tensor of t's shape whose axis order in memory follows t
 at::Tensor new_like_layout(const at::Tensor& t, const View& v) {
   if (t.size(1) > 1 && t.size(2) > 1 && v.st[1] < v.st[2]) return new_bnhd(t, t.size(0), t.size(1), t.size(2), t.size(3));
   return new_tensor(t.sizes(), t, t.scalar_type());
 }
-
-bool plain(const at::Tensor& t) {
-  // wrappers of function transforms, Python-dispatched and functional tensors keep to the general path
-  constexpr c10::DispatchKeySet special({c10::DispatchKey::FuncTorchGradWrapper, c10::DispatchKey::FuncTorchBatched,
-                                         c10::DispatchKey::FuncTorchVmapMode, c10::DispatchKey::Python,
-                                         c10::DispatchKey::Functionalize, c10::DispatchKey::Batched});
-  // (a forward-mode tangent too: the autograd functions of the general path refuse it, a result without one would be wrong)
-  return t.is_cuda() && t.layout() == at::kStrided && !t.key_set().has_any(special) && !t._fw_grad(/*level=*/0).defined();
-}
-
-// dispatch modes, and torch.jit.trace: the general path's autograd functions are recorded as operations of the graph, while
-// the output of a native call would be recorded as a constant
-bool modes_active() { return c10::impl::TorchDispatchModeTLS::any_modes_set() || at::tracer::impl::is_dispatch_enabled(); }
 
 struct Bias {
   at::Tensor t;               // fp32, contiguous: [B|1, H|1, N, N] up to leading axes of size 1
@@ -135,8 +58,6 @@ bool canonical_bias(const at::Tensor& bias, const Call& c, c10::Device dev, Bias
 }
 
 int64_t padded_rows(const Call& c) { return (static_cast<int64_t>(c.batch) * c.heads * c.n + 63) / 64 * 64; }
-
-c10::DataPtr workspace(int64_t bytes) { return c10::cuda::CUDACachingAllocator::get()->allocate(static_cast<size_t>(bytes)); }
 
 // row_m and row_z in one allocation, the second at a 256-byte boundary
 at::Tensor new_state(const Call& c, const at::Tensor& like) { return new_tensor({2 * padded_rows(c)}, like, at::kFloat); }
@@ -228,13 +149,6 @@ void bnhd_view(char* base, const Call& c, View* v) {
   v->st[0] = c.n * hd;
   v->st[1] = c.d;
   v->st[2] = hd;
-}
-
-// A saved tensor as the backward may use it: saved-tensor hooks may return the values in another memory layout (a copy
-// built from the sizes alone, an unaligned slice), so nothing but the values is taken for granted.
-void check_unpacked(const at::Tensor& t, at::IntArrayRef sizes, at::ScalarType dtype, c10::Device dev) {
-  TORCH_CHECK(t.defined() && plain(t) && t.device() == dev && t.scalar_type() == dtype && t.sizes() == sizes,
-              "a saved tensor of the attention came back from its unpack hook with another shape, dtype or device");
 }
 
 // what a backward needs beside the saved tensors
@@ -493,13 +407,6 @@ at::Tensor attention_packed(const at::Tensor& qkv, const at::Tensor& bias, Call 
 // ---- Python -----------------------------------------------------------------------------------
 // (positional arguments only: the Python operators resolve the keywords)
 
-bool get_tensor(PyObject* o, at::Tensor* t) {
-  if (o == Py_None) return true;
-  if (!THPVariable_CheckExact(o)) return false;
-  *t = THPVariable_Unpack(o);
-  return true;
-}
-
 bool get_call(PyObject* const* a, Call* c) {          // causal, summary dtype code, part_width, q_chunk
   const int causal = PyObject_IsTrue(a[0]);
   if (causal < 0) return false;
@@ -509,11 +416,6 @@ bool get_call(PyObject* const* a, Call* c) {          // causal, summary dtype c
   c->q_chunk = static_cast<int>(PyLong_AsLong(a[3]));
   return !PyErr_Occurred();
 }
-
-struct NoGil {
-  PyThreadState* s = PyEval_SaveThread();
-  ~NoGil() { PyEval_RestoreThread(s); }
-};
 
 // attention(q, k, v, bias, causal, summary, part_width, q_chunk, train)
 PyObject* py_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
@@ -553,7 +455,7 @@ PyObject* py_attention_packed(PyObject*, PyObject* const* a, Py_ssize_t n) {
 // bind({name: address}): the C ABI of the loaded library
 PyObject* py_bind(PyObject*, PyObject* d) {
   HANDLE_TH_ERRORS
-  auto at_name = [&](const char* name) -> void* {
+  const std::function<void*(const char*)> at_name = [&](const char* name) -> void* {
     PyObject* o = PyDict_GetItemString(d, name);
     TORCH_CHECK_VALUE(o != nullptr, "missing address of ", name);
     return PyLong_AsVoidPtr(o);
@@ -564,8 +466,9 @@ PyObject* py_bind(PyObject*, PyObject* d) {
   f_bwd_ws = reinterpret_cast<decltype(f_bwd_ws)>(at_name("elsa_backward_workspace_bytes"));
   f_bwd = reinterpret_cast<decltype(f_bwd)>(at_name("elsa_twopass_backward"));
   f_bwd_strided = reinterpret_cast<decltype(f_bwd_strided)>(at_name("elsa_twopass_backward_strided"));
-  f_strerror = reinterpret_cast<decltype(f_strerror)>(at_name("elsa_strerror"));
-  f_last_cuda_error = reinterpret_cast<decltype(f_last_cuda_error)>(at_name("elsa_last_cuda_error"));
+  elsa_host::f_strerror = reinterpret_cast<decltype(elsa_host::f_strerror)>(at_name("elsa_strerror"));
+  elsa_host::f_last_cuda_error = reinterpret_cast<decltype(elsa_host::f_last_cuda_error)>(at_name("elsa_last_cuda_error"));
+  elsa_host::bind_decoder(at_name);
   Py_RETURN_NONE;
   END_HANDLE_TH_ERRORS
 }
@@ -573,6 +476,9 @@ PyObject* py_bind(PyObject*, PyObject* d) {
 PyMethodDef kMethods[] = {
     {"attention", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_attention)), METH_FASTCALL, nullptr},
     {"attention_packed", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_attention_packed)), METH_FASTCALL, nullptr},
+    {"rotary", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(elsa_host::py_rotary)), METH_FASTCALL, nullptr},
+    {"shared_prefix", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(elsa_host::py_shared_prefix)), METH_FASTCALL, nullptr},
+    {"differential", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(elsa_host::py_differential)), METH_FASTCALL, nullptr},
     {"bind", py_bind, METH_O, nullptr},
     {nullptr, nullptr, 0, nullptr}};
 

@@ -1,7 +1,9 @@
-// fp32 products on the tensor cores' tf32 instruction (mma.sync m16n8k8): every operand x is taken as hi + lo, hi = x rounded to
-// tf32's 11 significant bits and lo the rest of it, rounded the same way, and a b = hi hi + hi lo + lo hi.  22 bits of each operand
-// take part: a product is right to about 2^-22 of its size, sums are fp32.  Three instructions of 1024 multiply-adds take the
-// place of 32 FMAs of each thread, and, what counts here, a quarter of their shared-memory reads.
+// fp32 products on the tensor cores' tf32 instruction (mma.sync m16n8k8, which reads the upper 19 bits of its operands): every operand x
+// is taken as hi + lo, hi = x cut to tf32's 11 significant bits and lo = x - hi (exact), rounded to as many, and a b = hi hi + hi lo +
+// lo hi.  lo is below 2^-10 of x, so an operand is right to 2^-21 of its size and what is left out, lo lo, is below 2^-20 of the
+// product and 2^-22 of it on average; sums are fp32.  (Both parts rounded would be better by a third and take 131 us where this takes
+// 125, for dQ at (1, 4 heads, 1000 tokens, 64 / 128, causal); cvt.rna, which runs at a fraction of the ALU's rate, 145.)  Three
+// instructions of 1024 multiply-adds take the place of 32 FMAs of each thread and a quarter of their shared-memory reads.
 #pragma once
 
 #include "common.cuh"
@@ -13,19 +15,23 @@ struct Split { uint32_t hi, lo; };
 
 __device__ __forceinline__ Split split(float x) {
   Split s;
-  asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(s.hi) : "f"(x));
-  asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(s.lo) : "f"(x - __uint_as_float(s.hi)));
+  s.hi = __float_as_uint(x) & 0xffffe000u;
+  s.lo = __float_as_uint(x - __uint_as_float(s.hi)) + 0x1000u;      // (half a step of tf32: the instruction's cut rounds)
   return s;
 }
 __device__ __forceinline__ void mma(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
   asm volatile("mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
-// d[16 x 8] += a[16 x 8] b[8 x 8]
+// d[16 x 8] += a[16 x 8] b[8 x 8].  The instruction cuts its sums instead of rounding them, always towards zero: three of them in a row are
+// added to the running sum by an FADD, which rounds (a chain of them over 1000 keys lost 2 bits: 3.9e-6 against 8e-7 for dK).
 __device__ __forceinline__ void mma3(float (&d)[4], const Split (&a)[4], const Split (&b)[2]) {
-  mma(d, a[0].lo, a[1].lo, a[2].lo, a[3].lo, b[0].hi, b[1].hi);
-  mma(d, a[0].hi, a[1].hi, a[2].hi, a[3].hi, b[0].lo, b[1].lo);
-  mma(d, a[0].hi, a[1].hi, a[2].hi, a[3].hi, b[0].hi, b[1].hi);
+  float t[4] = {0.f, 0.f, 0.f, 0.f};
+  mma(t, a[0].lo, a[1].lo, a[2].lo, a[3].lo, b[0].hi, b[1].hi);
+  mma(t, a[0].hi, a[1].hi, a[2].hi, a[3].hi, b[0].lo, b[1].lo);
+  mma(t, a[0].hi, a[1].hi, a[2].hi, a[3].hi, b[0].hi, b[1].hi);
+#pragma unroll
+  for (int e = 0; e < 4; ++e) d[e] += t[e];
 }
 
 // Fragments of a warp's lane (r = lane / 4, q = lane % 4).  Matrices stand in shared memory row by row; a pitch of 4 mod 32 floats

@@ -11,7 +11,8 @@ from typing import Optional, Union
 import torch
 
 from . import _lib
-from .attention import _DeviceScope, _cached_bytes, _in_place_or_copy
+from .attention import _DeviceScope, _aligned, _cached_bytes, _in_place_or_copy
+from .rotary import _check_saved, _once_differentiable
 from .shared_prefix import _check_lengths, _positive_scale, _readable, _strides
 
 
@@ -108,6 +109,13 @@ def differential_attention(
     nothing behind them is read).  A query without any key gives zeros.  D, Dv <= 128; fp16, bf16 or fp32; rows of contiguous
     elements are read in place.  scale: 1 / sqrt(D) by default.  Forward only: see `differential_attention_train`.
     Returns [B, H, Nq, Dv]."""
+    if isinstance(q, torch.Tensor) and q.is_cuda:
+        host = _lib.host()
+        if host is not None:
+            out = host.differential(q, k, v, lam, is_causal, scale, lengths, False) if isinstance(lam, torch.Tensor) else None
+            if out is not None:
+                return out
+    # the general path: what the native one does not cover, and the errors
     sizes = _check(q, k, v, lam, "differential_attention")
     _check_lengths(lengths, sizes[0], q.device)
     scale = _positive_scale(scale, sizes[5])
@@ -117,8 +125,8 @@ def differential_attention(
 
 
 def _for_tiles(t):
-    """As the tensor-core kernels read it, in place or copied; other types and head dims as they are."""
-    return _in_place_or_copy(t)[0] if t.dtype != torch.float32 and t.shape[-1] % 8 == 0 and t.numel() else t
+    """Rows on 16-byte boundaries, in place or copied; other head dims as they are."""
+    return _in_place_or_copy(t)[0] if t.shape[-1] % 8 == 0 and t.numel() else t
 
 
 class _DifferentialAutograd(torch.autograd.Function):
@@ -126,14 +134,18 @@ class _DifferentialAutograd(torch.autograd.Function):
     def forward(ctx, q, k, v, lam, sizes, is_causal, scale):
         out, out2, lse, q, k, v = _forward(_for_tiles(q), _for_tiles(k), _for_tiles(v), lam, sizes, is_causal, scale, None, True)
         ctx.lam = None if isinstance(lam, torch.Tensor) else lam
-        ctx.save_for_backward(q, k, v, out, out2, lse, *((lam,) if isinstance(lam, torch.Tensor) else ()))
+        kept = (q, k, v, out, out2, lse, *((lam,) if isinstance(lam, torch.Tensor) else ()))
+        ctx.save_for_backward(*kept)
+        ctx.kept = [(t.shape, t.dtype, t.device) for t in kept]
         ctx.sizes, ctx.is_causal, ctx.scale = sizes, is_causal, scale
         return out
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
+    @_once_differentiable
     def backward(ctx, dout):
-        q, k, v, out, out2, lse, *rest = ctx.saved_tensors
+        q, k, v, out, out2, lse, *rest = (_check_saved(t, *kept) for t, kept in zip(ctx.saved_tensors, ctx.kept))
+        (q, _), (k, _), (v, _), (out, _) = (_readable(_for_tiles(t)) for t in (q, k, v, out))
+        out2, lse = _aligned(out2), _aligned(lse)
         lam = rest[0] if rest else ctx.lam
         batch, heads, kv_heads, nq, nk, dim, v_dim = ctx.sizes
         dout, gs = _readable(_for_tiles(dout.to(q.dtype)))
@@ -169,6 +181,13 @@ def differential_attention_train(
     """Differentiable `differential_attention` (without lengths), in q, k, v and, where it is a tensor, lam: the forward keeps P2 v and each
     row's log sum, the backward recomputes the maps.  Gradients repeat bit for bit; those of shared key heads and of a shared lam are
     summed."""
+    if isinstance(q, torch.Tensor) and q.is_cuda:
+        host = _lib.host()
+        if host is not None:
+            out = host.differential(q, k, v, lam, is_causal, scale, None, True) if isinstance(lam, torch.Tensor) else None
+            if out is not None:
+                return out
+    # the general path: what the native one does not cover, and the errors
     sizes = _check(q, k, v, lam, "differential_attention_train")
     scale = _positive_scale(scale, sizes[5])
     if any(x == 0 for x in (sizes[0], sizes[1], sizes[3], sizes[4], sizes[6])):

@@ -6,6 +6,7 @@ The reference has no position encoding of this kind; names and checks follow thi
 from __future__ import annotations
 
 import ctypes
+import functools
 import math
 from typing import Literal, Optional, Union
 
@@ -134,22 +135,46 @@ def _rotate(q, k, frequencies, positions, magnitude, interleaved, inverse=False,
     return q_out, k_out
 
 
+def _check_saved(t, like_shape, dtype, device):
+    """Saved-tensor hooks may return the values in another memory layout, but nothing else."""
+    if tuple(t.shape) != tuple(like_shape) or t.dtype != dtype or t.device != device:
+        raise RuntimeError("a saved tensor came back from its unpack hook with another shape, dtype or device")
+    return t
+
+
+def _once_differentiable(backward):
+    """A backward whose results have no gradients of their own, and say so when one is asked for."""
+
+    @functools.wraps(backward)
+    def wrapper(ctx, *grads):
+        record = torch.is_grad_enabled()
+        with torch.no_grad():
+            out = backward(ctx, *grads)
+        if not record:
+            return out
+        error = torch._C._functions.DelayedError(b"this gradient is not differentiable twice", len(out))
+        return error(*(None if t is None else t.detach().requires_grad_() for t in out))
+
+    return wrapper
+
+
 class _RotaryAutograd(torch.autograd.Function):
     """The gradient of a rotation is the rotation back: nothing but positions and frequencies is kept."""
 
     @staticmethod
     def forward(ctx, q, k, frequencies, positions, magnitude, interleaved):
         ctx.save_for_backward(frequencies, *(() if positions is None else (positions,)))
+        ctx.kept = [(t.shape, t.dtype, t.device) for t in (frequencies, *(() if positions is None else (positions,)))]
         ctx.magnitude, ctx.interleaved = magnitude, interleaved
         ctx.set_materialize_grads(False)
         q_out, k_out = _rotate(q, k, frequencies, positions, magnitude, interleaved)
         return q_out if k is None else (q_out, k_out)
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
+    @_once_differentiable
     def backward(ctx, dq, dk=None):
-        frequencies, *rest = ctx.saved_tensors
-        positions = rest[0] if rest else None
+        frequencies, *rest = (_check_saved(t, *kept) for t, kept in zip(ctx.saved_tensors, ctx.kept))
+        frequencies, positions = frequencies.contiguous(), rest[0] if rest else None
         back = (frequencies, positions, ctx.magnitude, ctx.interleaved, True)
         if not ctx.needs_input_grad[0]:
             dq = None
@@ -181,6 +206,13 @@ def rotary_embedding(
     `rotary_frequencies`, with its `magnitude`.  positions: int32 or int64, [N] or [B, N], any values; None: 0 .. N-1.
     Dimension i is paired with i + R/2, or, with `interleaved`, 2i with 2i + 1; dimensions from R on stay as they are.
     Differentiable in q and k.  `inplace` writes over q and k instead (no gradients then).  Returns q', or (q', k')."""
+    if not inplace and isinstance(q, torch.Tensor) and q.is_cuda:
+        host = _lib.host()
+        if host is not None:
+            out = host.rotary(q, k, frequencies, positions, interleaved, magnitude)
+            if out is not None:
+                return out
+    # the general path: what the native one does not cover, and the errors
     if q.dim() != 4 or (k is not None and k.dim() != 4):
         raise ValueError("q, k must have shape [B,H,N,D]")
     if k is not None and (k.shape[0] != q.shape[0] or k.shape[2:] != q.shape[2:]):
@@ -217,7 +249,4 @@ def rotary_embedding(
         _rotate(q, k, frequencies, positions, magnitude, interleaved, inplace=True)
         torch.autograd.graph.increment_version((q,) if k is None else (q, k))     # (what a graph had saved is gone)
         return q if k is None else (q, k)
-    if torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad)):
-        return _RotaryAutograd.apply(q, k, frequencies, positions, magnitude, bool(interleaved))
-    q_out, k_out = _rotate(q, k, frequencies, positions, magnitude, interleaved)
-    return q_out if k is None else (q_out, k_out)
+    return _RotaryAutograd.apply(q, k, frequencies, positions, magnitude, bool(interleaved))

@@ -64,6 +64,13 @@ def shared_prefix_attention(
     heads share a key head.  P or S may be 0; a query without any key gives zeros.  D <= 128; fp16, bf16 or fp32; rows of D
     contiguous elements are read in place, whatever the other strides.  scale: 1 / sqrt(D) by default.  Forward only.
     Returns [B, H, Nq, D]."""
+    if isinstance(q, torch.Tensor) and q.is_cuda:
+        host = _lib.host()
+        if host is not None:
+            out = host.shared_prefix(q, k_prefix, v_prefix, k, v, lengths, scale)
+            if out is not None:
+                return out
+    # the general path: what the native one does not cover, and the errors
     if q.dim() != 4 or k.dim() != 4 or v.dim() != 4:
         raise ValueError("q, k, v must have shape [B,H,N,D]")
     if k_prefix.dim() != 3 or v_prefix.dim() != 3:
