@@ -21,7 +21,7 @@ HOST_HEADER = os.path.join(CSRC, "host_common.h")
 HOST_PATH = os.path.join(HERE, "_host.so")
 HOST_STAMP = os.path.join(OBJ_DIR, "_host.built_for")
 SOURCES = ["api.cu", "phase2.cu", "fold_simt.cu", "bwd_simt.cu", "fold_tc.cu", "fold_tc3.cu", "fold_tcw.cu", "bwd_tc.cu", "bwd_tc3.cu", "bwd_tcw.cu", "win_tc.cu", "peaks.cu",
-           "api_decoder.cu", "decode.cu", "diff_tc.cu", "diff_bwd_tc.cu", "diff_any.cu",
+           "api_decoder.cu", "decode.cu", "pair_tc.cu", "diff_bwd_tc.cu", "diff_any.cu",
            "rotary.cu"]
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17",

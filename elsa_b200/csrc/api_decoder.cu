@@ -5,6 +5,7 @@
 #include "decode.cuh"
 #include "diff.cuh"
 #include "kernels.cuh"
+#include "pair_tc.cuh"
 
 using namespace elsa;
 
@@ -34,14 +35,14 @@ int split_width(int64_t blocks_of_one_split, int n_keys) {
 
 // ---- attention over a shared prefix ------------------------------------------------------------------------------------
 struct PrefixPlan {
-  bool fold;                    // the prefix on the 128- and 256-row tensor-core fold (fold_tc.cu, fold_tcw.cu)
+  bool tiles;                   // the prefix on the 256-row tensor-core kernel (pair_tc.cu)
   int prefix_width, prefix_parts, own_width, own_parts;
-  int64_t rows, q_bytes, mz_bytes, s_bytes;
-  int64_t bytes() const { return q_bytes + 2 * mz_bytes + s_bytes; }
+  int64_t rows, mz_bytes, s_bytes;
+  int64_t bytes() const { return 2 * mz_bytes + s_bytes; }
 };
 
 // More rows for each key head than two 16-row tiles: the split kernel would read the prefix once for each tile.
-constexpr int kFoldRows = 32;
+constexpr int kTileRows = 32;
 
 int plan_prefix(int dtype, int batch, int heads, int kv_heads, int nq, int head_dim, int n_prefix, int n_own, PrefixPlan* pl) {
   if (!dtype_ok(dtype) || batch < 1 || heads < 1 || kv_heads < 1 || heads % kv_heads || nq < 1 || head_dim < 1 || n_prefix < 0 || n_own < 0)
@@ -50,29 +51,27 @@ int plan_prefix(int dtype, int batch, int heads, int kv_heads, int nq, int head_
   const int64_t rows = static_cast<int64_t>(batch) * (heads / kv_heads) * nq;
   if (rows * heads > 0x3fffffff || kv_heads > 65535 || n_prefix > 0x3fffffff || n_own > 0x3fffffff) return ELSA_ERR_UNSUPPORTED;
   pl->rows = rows;
-  pl->fold = rows > kFoldRows && n_prefix >= 128 && (fold_tc_supported(dtype, head_dim, false) || fold_tcw_supported(dtype, head_dim, false));
+  pl->tiles = rows > kTileRows && n_prefix >= 128 && (fold_tc_supported(dtype, head_dim, false) || fold_tcw_supported(dtype, head_dim, false));
   pl->prefix_width = pl->prefix_parts = pl->own_width = pl->own_parts = 0;
   if (n_own > 0) {
     pl->own_width = split_width(static_cast<int64_t>(batch) * kv_heads * cdiv64(heads / kv_heads * nq, 16), n_own);
     pl->own_parts = static_cast<int>(cdiv64(n_own, pl->own_width));
   }
-  if (pl->fold) {
-    // one CTA for each row tile, key head and part, one CTA on an SM: waves x (key tiles of a part + what a CTA costs besides, about
-    // four of them)
-    const int tile = head_dim <= 64 ? 256 : 128;
-    const int64_t ctas = cdiv64(rows, tile) * kv_heads, tiles = cdiv64(n_prefix, 128);
+  if (pl->tiles) {
+    // one CTA for each 256 rows, key head and part, one CTA on an SM: waves x (64-key tiles of a part + what a CTA costs besides, about
+    // eight of them)
+    const int64_t ctas = cdiv64(rows, 256) * kv_heads, tiles = cdiv64(n_prefix, 64);
     int64_t best = 0, best_cost = 0;
     for (int64_t parts = 1; parts <= std::min<int64_t>(tiles, 64); ++parts) {
-      const int64_t per = cdiv64(tiles, parts), cost = cdiv64(ctas * cdiv64(tiles, per), sm_count()) * (per + 4);
+      const int64_t per = cdiv64(tiles, parts), cost = cdiv64(ctas * cdiv64(tiles, per), sm_count()) * (per + 8);
       if (best == 0 || cost < best_cost) { best = per; best_cost = cost; }
     }
-    pl->prefix_width = static_cast<int>(best * 128);
+    pl->prefix_width = static_cast<int>(best * 64);
   } else if (n_prefix > 0) {
     pl->prefix_width = split_width(kv_heads * cdiv64(rows, 16), n_prefix);
   }
   if (n_prefix > 0) pl->prefix_parts = static_cast<int>(cdiv64(n_prefix, pl->prefix_width));
   const int64_t summaries = static_cast<int64_t>(pl->prefix_parts + pl->own_parts) * kv_heads * rows;
-  pl->q_bytes = pl->fold ? align_up(rows * kv_heads * head_dim * 2, 256) : 0;
   pl->mz_bytes = align_up(summaries * 4, 256);
   pl->s_bytes = align_up(summaries * head_dim * 4, 256);
   return ELSA_OK;
@@ -80,7 +79,7 @@ int plan_prefix(int dtype, int batch, int heads, int kv_heads, int nq, int head_
 
 // ---- differential attention -------------------------------------------------------------------------------------------
 struct DiffPlan {
-  bool tensor_tiles;            // the 128-row tensor-core kernels by sizes (diff_tc.cu); else the split kernels (decode.cu)
+  bool tensor_tiles;            // the 128-row tensor-core kernels by sizes (pair_tc.cu); else the split kernels (decode.cu)
   int split_width, parts;       // of the split kernels
   int64_t mz_bytes, s_bytes;
   int64_t bytes() const { return 2 * mz_bytes + s_bytes; }
@@ -162,37 +161,25 @@ extern "C" int elsa_shared_prefix_attention(const void* q, const void* k_prefix,
   p.q = q; p.qs = Strides{strides[0], strides[1], strides[2]};
   p.batch = batch; p.heads = heads; p.kv_heads = kv_heads; p.nq = nq; p.head_dim = p.v_dim = head_dim; p.maps = 1;
   p.scale_log2 = static_cast<float>(scale * 1.4426950408889634);
-  p.m = reinterpret_cast<float*>(ws + pl.q_bytes);
-  p.z = reinterpret_cast<float*>(ws + pl.q_bytes + pl.mz_bytes);
-  p.s = reinterpret_cast<float*>(ws + pl.q_bytes + 2 * pl.mz_bytes);
+  p.m = reinterpret_cast<float*>(ws);
+  p.z = reinterpret_cast<float*>(ws + pl.mz_bytes);
+  p.s = reinterpret_cast<float*>(ws + 2 * pl.mz_bytes);
   p.out = out; p.os = Strides{strides[13], strides[14], strides[15]};
-  const Strides kps{0, strides[3], strides[4]}, vps{0, strides[5], strides[6]};
-  bool fold = pl.fold;
-  if (fold) {
-    // what tensor maps ask of the prefix; another layout goes through the split kernel with the same parts
-    fold = !((kps.h | kps.r | vps.h | vps.r) & 7) && kps.r >= head_dim && vps.r >= head_dim && (kv_heads == 1 || (kps.h > 0 && vps.h > 0)) &&
-           !((reinterpret_cast<uintptr_t>(k_prefix) | reinterpret_cast<uintptr_t>(v_prefix)) & 15u);
-  }
-  if (fold) {
-    if ((rc = device_status_ok()) != ELSA_OK) return rc;
-    if ((rc = decode_pack_q(p, ws, st)) != ELSA_OK) return rc;
-    FoldParams f{};
-    f.q = ws; f.k = k_prefix; f.v = v_prefix;
-    f.qs = contiguous_strides(kv_heads, pl.rows, head_dim); f.ks = kps; f.vs = vps;
-    f.m = p.m; f.z = p.z; f.s = p.s;
-    f.heads = f.bh = kv_heads; f.n_ctx = f.q_len = static_cast<int>(pl.rows); f.head_dim = head_dim;
-    f.part_width = pl.prefix_width; f.n_parts = pl.prefix_parts; f.n_keys = n_prefix;
-    f.summary_dtype = ELSA_F32;
-    f.scale = static_cast<float>(scale); f.scale_log2 = p.scale_log2;
-    rc = head_dim <= 64 ? fold_tc(f, dtype, st) : fold_tcw(f, dtype, st);
-    if (rc != ELSA_OK) return rc;
-  } else if (n_prefix > 0) {
-    DecodeSegment& s = p.seg[p.n_segs++];
-    s.k = k_prefix; s.v = v_prefix; s.ks = kps; s.vs = vps; s.n_keys = n_prefix; s.shared = 1;
+  if (n_prefix > 0) {
+    DecodeSegment& s = p.seg[0];
+    s.k = k_prefix; s.v = v_prefix; s.ks = Strides{0, strides[3], strides[4]}; s.vs = Strides{0, strides[5], strides[6]}; s.n_keys = n_prefix; s.shared = 1;
     s.split_width = pl.prefix_width; s.n_splits = pl.prefix_parts; s.first_part = 0;
+    // (a layout that the tensor maps do not take goes through the split kernel with the same parts)
+    if (pl.tiles && rows_tc_ok(p, dtype)) {
+      if ((rc = device_status_ok()) != ELSA_OK) return rc;
+      if ((rc = rows_tc(p, pl.prefix_width, pl.prefix_parts, dtype, st)) != ELSA_OK) return rc;
+    } else {
+      p.n_segs = 1;
+    }
   }
   if (n_own > 0) {
     DecodeSegment& s = p.seg[p.n_segs++];
+    s = DecodeSegment{};
     s.k = k; s.v = v; s.ks = Strides{strides[7], strides[8], strides[9]}; s.vs = Strides{strides[10], strides[11], strides[12]};
     s.lengths = lengths; s.n_keys = n_own; s.causal = 1;
     s.split_width = pl.own_width; s.n_splits = pl.own_parts; s.first_part = pl.prefix_parts;

@@ -552,18 +552,6 @@ merge_kernel(const DecodeParams p, int n_parts) {
   }
 }
 
-// q as [kv head][row][head_dim], E the elements of one access
-template <typename E>
-__global__ void __launch_bounds__(256)
-pack_q_kernel(const DecodeParams p, E* packed, int row_elements) {
-  const int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
-  const int rows = static_cast<int>(decode_rows(p));
-  if (i >= static_cast<int64_t>(rows) * p.kv_heads * row_elements) return;
-  const int gr = static_cast<int>(i / row_elements), col = static_cast<int>(i - static_cast<int64_t>(gr) * row_elements);
-  const int g = gr / rows, row = gr - g * rows;
-  packed[i] = reinterpret_cast<const E*>(static_cast<const __half*>(p.q) + q_offset(p, g, row, 0))[col];
-}
-
 template <typename T, int MAPS, int DP, int VP>
 int launch_mma(const DecodeParams& p, int64_t blocks, cudaStream_t st) {
   const auto kernel = &split_mma_kernel<T, MAPS, DP, VP>;
@@ -623,19 +611,6 @@ int decode_split(DecodeParams& p, int dtype, cudaStream_t st) {
   if (mma) return dtype == ELSA_F16 ? launch_mma_t<__half>(p, blocks, st) : launch_mma_t<__nv_bfloat16>(p, blocks, st);
   if (dtype == ELSA_F32) return launch_any_t<float>(p, blocks, st);
   return dtype == ELSA_F16 ? launch_any_t<__half>(p, blocks, st) : launch_any_t<__nv_bfloat16>(p, blocks, st);
-}
-
-int decode_pack_q(const DecodeParams& p, void* packed, cudaStream_t st) {
-  if (p.maps != 1) return ELSA_ERR_UNSUPPORTED;
-  const bool wide = p.head_dim % 8 == 0 && !((p.qs.b | p.qs.h | p.qs.r) & 7) && !(reinterpret_cast<uintptr_t>(p.q) & 15u);
-  const int row_elements = wide ? p.head_dim / 8 : p.head_dim;
-  const int64_t blocks = cdiv64(decode_rows(p) * p.kv_heads * row_elements, 256);
-  if (blocks > 0x7fffffffll) return ELSA_ERR_UNSUPPORTED;
-  // (16-bit elements are moved, not looked at)
-  if (wide) pack_q_kernel<uint4><<<static_cast<unsigned>(blocks), 256, 0, st>>>(p, static_cast<uint4*>(packed), row_elements);
-  else pack_q_kernel<uint16_t><<<static_cast<unsigned>(blocks), 256, 0, st>>>(p, static_cast<uint16_t*>(packed), row_elements);
-  ELSA_LAUNCH_CHECK();
-  return ELSA_OK;
 }
 
 template <typename T>

@@ -42,8 +42,6 @@ __host__ __device__ inline int64_t decode_rows(const DecodeParams& p) { return s
 bool decode_mma_ok(const DecodeParams& p, int dtype);
 // summaries of all segments in one launch; parts that begin beyond a sequence's keys are not written
 int decode_split(DecodeParams& p, int dtype, cudaStream_t st);
-// q of 16-bit elements (one map) as [kv head][row][head_dim]
-int decode_pack_q(const DecodeParams& p, void* packed, cudaStream_t st);
 // all parts of a row merged (of a segment that is not shared: those that begin before the sequence's last key)
 int decode_merge(const DecodeParams& p, int n_parts, int dtype, cudaStream_t st);
 

@@ -25,7 +25,6 @@ struct DiffParams {
 // sizes that the tcgen05 kernels take (16-bit types), and the strides and addresses that their tensor maps ask for
 bool diff_tc_sizes(int dtype, int head_dim, int v_dim);
 bool diff_rows_ok(const void* base, const Strides& s, int row, int heads, int batch);
-int diff_tc_fwd(const DiffParams& p, int dtype, cudaStream_t st);
 // row statistics of the backward, [B * heads][-LSE1, -LSE2, -D1, -D2][n_pad] with n_pad = nq rounded up to 128, and dlam (diff_any.cu)
 inline int64_t diff_stats_bytes(int batch, int heads, int nq) { return static_cast<int64_t>(batch) * heads * 4 * align_up(nq, 128) * 4; }
 int diff_stats(const DiffParams& p, float* stats, int dtype, cudaStream_t st);
