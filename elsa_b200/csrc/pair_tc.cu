@@ -8,14 +8,14 @@
 //   warp 8      TMA producer
 //   warp 9, 10  MMA issuers   one for each chain t:  S_t(j) = Q_t K_t^T   (tcgen05.mma 128x64x16, shared-memory operands)
 //                                                    O_t   += P_t V       (tcgen05.mma 128xDx16, P from TMEM, V MN-major)
-//   warps 0-3   fold of chain 0  one thread per query row: 64 scores into registers, running max, exp2, row sum, P (16-bit) over the
-//   warps 4-7   fold of chain 1  columns that the scores came from, rescale of O when the max moved
+//   warps 0-3   fold of chain 0  one thread per query row: 64 scores into registers, running max, exp2, row sum, P (16-bit) into TMEM,
+//   warps 4-7   fold of chain 1  rescale of O when the max moved
 //
-// TMEM columns: chain t has two score tiles S_t[2] at 128 t, tile j in S_t[j % 2] (P over its first 32 columns), and O_t at 256 + 128 t.
-// The scores of tile j + 2 are issued behind P V of tile j, over the P that it reads, while the fold works on tile j + 1: a fold warp
-// finds its scores ready and waits for the tensor pipe only when its maximum moves.  (With 128-key tiles one S_t fits beside O_t, the
-// next scores wait for P V, and scores, exponentials and P V of a chain follow one another: 3650 cycles for 128 keys of both chains,
-// (2, 8, 8192, 64 / 128) causal 460 us.)
+// TMEM columns: chain t has S_t at 128 t, two tiles of P_t at 128 t + 64 and + 96, and O_t at 256 + 128 t.  S_t(j + 1) is issued as soon as the
+// fold holds S_t(j) in registers and runs during the exponentials of tile j; a fold warp waits for the tensor pipe only when its
+// maximum moves.  Measured, (2, 8, 8192, 64 / 128) causal bf16: 128-key tiles, whose P has no columns of its own, so that scores,
+// exponentials and P V of a chain follow one another, 460 us; 64-key tiles with two S_t, P over the scores it comes from, 460 (the
+// scores of tile j + 1 wait for P V of tile j - 1); the latter with the next scores read ahead of the exponentials 550.
 //
 // Bound: the ex2 unit, 2 x 128 x 64 exponentials for each tile (1024 cycles; the tensor pipe, limited by its shared-memory operands,
 // needs 900 for Diff and 1280 for Rows128).
@@ -55,7 +55,7 @@ template <int MODE> struct Shape {
   static constexpr int kSmem = 2 * kQHalves * kTileBytes + kStages * kStageBytes + 1024;   // + alignment slack
 };
 
-enum BarId { BAR_Q = 71, BAR_KV_FULL = 72, BAR_KV_FREE = 73, BAR_S = 74, BAR_P = 75, BAR_PV = 76, BAR_STAGGER = 77, BAR_O = 78 };
+enum BarId { BAR_Q = 71, BAR_KV_FULL = 72, BAR_KV_FREE = 73, BAR_S = 74, BAR_P = 75, BAR_PV = 76, BAR_STAGGER = 77, BAR_O = 78, BAR_SFREE = 79 };
 
 struct PairParams {
   DiffParams d;                  // Diff
@@ -132,9 +132,10 @@ pair_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant__ 
   const uint32_t bar_q = bar0, bar_stagger = bar0 + 8;
   auto bar_kv_full = [&](int st) { return bar0 + 8 * (2 + st); };
   auto bar_kv_free = [&](int st) { return bar0 + 8 * (2 + kStages + st); };
-  // one of each for either score tile: the one of tile j + 1 can complete before the last thread has seen tile j's
-  auto bar_s = [&](int t, int b) { return bar0 + 8 * (2 + 2 * kStages + 2 * t + b); };     // S_t(j) is in TMEM
-  auto bar_p = [&](int t, int b) { return bar0 + 8 * (6 + 2 * kStages + 2 * t + b); };     // P_t(j) has been delivered
+  auto bar_s = [&](int t) { return bar0 + 8 * (2 + 2 * kStages + t); };                    // S_t(j) is in TMEM
+  auto bar_sfree = [&](int t) { return bar0 + 8 * (4 + 2 * kStages + t); };                // the fold warps hold it in registers
+  // P_t(j) has been delivered: one for either tile, because P_t(j + 1) can be there before the issuer has looked at P_t(j)'s
+  auto bar_p = [&](int t, int b) { return bar0 + 8 * (6 + 2 * kStages + 2 * t + b); };
   auto bar_pv = [&](int t) { return bar0 + 8 * (10 + 2 * kStages + t); };                  // P_t V of tile j has retired
   auto bar_o = [&](int t) { return bar0 + 8 * (12 + 2 * kStages + t); };                   // ... of the last tile
 
@@ -144,7 +145,8 @@ pair_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant__ 
     mbar_init(bar_stagger, 1);
     for (int st = 0; st < kStages; ++st) { mbar_init(bar_kv_full(st), 1); mbar_init(bar_kv_free(st), 2); }
     for (int t = 0; t < 2; ++t) {
-      for (int b = 0; b < 2; ++b) { mbar_init(bar_s(t, b), 1); mbar_init(bar_p(t, b), 4); }
+      mbar_init(bar_s(t), 1); mbar_init(bar_sfree(t), 4);
+      for (int b = 0; b < 2; ++b) mbar_init(bar_p(t, b), 4);
       mbar_init(bar_pv(t), 1); mbar_init(bar_o(t), 1);
     }
     fence_mbar_init();
@@ -157,7 +159,8 @@ pair_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant__ 
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem_base = tmem_base_slot;
-  auto tS = [&](int t, int b) { return tmem_base + 128 * t + 64 * b; };
+  auto tS = [&](int t) { return tmem_base + 128 * t; };
+  auto tP = [&](int t, int b) { return tmem_base + 128 * t + 64 + 32 * b; };
   auto tO = [&](int t) { return tmem_base + 256 + 128 * t; };
 
   // registers: 3 x 128 threads, 232 + 232 + 40 = 3 x 168, the launch allocation (see fold_tc.cu)
@@ -196,26 +199,28 @@ pair_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant__ 
       auto issue_s = [&](int j) {
         const int st = j % kStages;
         if (!(ok = mbar_wait_warp(bar_kv_full(st), (j / kStages) & 1, &abort_flag, prm.status, BAR_KV_FULL))) return;
+        if (j > 0 && !(ok = mbar_wait_warp(bar_sfree(t), (j - 1) & 1, &abort_flag, prm.status, BAR_SFREE))) return;
         tc_fence_after();
 #pragma unroll
         for (int h = 0; h < Sh::kQHalves; ++h)
-          if (leader) mma_ss_x4<2, 2>(tS(t, j & 1), dq + h * (kTileBytes >> 4), dk0 + st * kStageStep + h * (kSlotBytes >> 4), idesc_s, h == 0 ? 0u : 1u);
-        if (leader) mma_commit(bar_s(t, j & 1));
+          if (leader) mma_ss_x4<2, 2>(tS(t), dq + h * (kTileBytes >> 4), dk0 + st * kStageStep + h * (kSlotBytes >> 4), idesc_s, h == 0 ? 0u : 1u);
+        if (leader) mma_commit(bar_s(t));
       };
       // chain 1 starts half a period after chain 0: in step they would want the ex2 unit at the same time
       if (ok && t == 1) ok = mbar_wait_warp(bar_stagger, 0, &abort_flag, prm.status, BAR_STAGGER);
       if (ok) issue_s(0);
-      if (ok && n_t > 1) issue_s(1);
       for (int j = 0; ok && j < n_t; ++j) {
         const int st = j % kStages;
-        if (!(ok = mbar_wait_warp(bar_p(t, j & 1), (j >> 1) & 1, &abort_flag, prm.status, BAR_P))) break;
+        if (j + 1 < n_t) {
+          issue_s(j + 1);
+          if (!ok) break;
+        }
         if (t == 0 && j == 0 && leader) mbar_arrive(bar_stagger);
+        if (!(ok = mbar_wait_warp(bar_p(t, j & 1), (j >> 1) & 1, &abort_flag, prm.status, BAR_P))) break;
         tc_fence_after();
-        if (leader) mma_ts_x4<8, 128>(tO(t), tS(t, j & 1), dv0 + st * kStageStep, idesc_o, j > 0 ? 1u : 0u);
+        if (leader) mma_ts_x4<8, 128>(tO(t), tP(t, j & 1), dv0 + st * kStageStep, idesc_o, j > 0 ? 1u : 0u);
         if (leader) mma_commit(bar_pv(t));
         if (leader) mma_commit(bar_kv_free(st));  // this chain no longer reads the stage
-        // scores of tile j + 2 over P(j): the tensor pipe takes them after the P V that reads it
-        if (j + 2 < n_t) issue_s(j + 2);
       }
       if (ok && leader) mma_commit(bar_o(t));
     }
@@ -252,14 +257,17 @@ pair_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant__ 
     const int lim = MODE == kDiff && p.causal ? min(p.nk - 1, qi + shift) : k_end - 1;
 
     for (int j = 0; j < n_t; ++j) {
-      if (!mbar_wait_warp(bar_s(t, j & 1), (j >> 1) & 1, &abort_flag, prm.status, BAR_S)) { alive = false; break; }
+      // (S(j) was issued behind P V of tile j - 2: its P may be overwritten)
+      if (!mbar_wait_warp(bar_s(t), j & 1, &abort_flag, prm.status, BAR_S)) { alive = false; break; }
       tc_fence_after();
       float sv[64];
       {
         uint32_t ra[32], rb[32];
-        tmem_ld32(tS(t, j & 1) + lane_off, ra);
-        tmem_ld32(tS(t, j & 1) + lane_off + 32, rb);
+        tmem_ld32(tS(t) + lane_off, ra);
+        tmem_ld32(tS(t) + lane_off + 32, rb);
         tmem_wait_ld();
+        tc_fence_before();
+        mbar_arrive_warp(bar_sfree(t), lane);      // S_t may be overwritten with the next tile's scores
 #pragma unroll
         for (int i = 0; i < 32; ++i) { sv[i] = __uint_as_float(ra[i]); sv[32 + i] = __uint_as_float(rb[i]); }
       }
@@ -309,7 +317,7 @@ pair_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant__ 
         ps[i & 3] = __fadd2_rn(ps[i & 3], pp);
         pk[i] = pack2<T>(pp.x, pp.y);
       }
-      tmem_st32(tS(t, j & 1) + lane_off, pk);
+      tmem_st32(tP(t, j & 1) + lane_off, pk);
       tmem_wait_st();               // (also covers the O rescale stores above)
       tc_fence_before();
       mbar_arrive_warp(bar_p(t, j & 1), lane);
