@@ -60,6 +60,9 @@ __device__ __forceinline__ void st_shared_v4(uint32_t addr, uint32_t a, uint32_t
   asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
 }
 
+__device__ __forceinline__ float2 pair(const uint32_t (&r)[16], int i) { return make_float2(__uint_as_float(r[i]), __uint_as_float(r[i + 1])); }
+__device__ __forceinline__ float2 exp2_pair(float2 x) { return make_float2(fast_exp2(x.x), fast_exp2(x.y)); }
+
 // the first n (a multiple of 8, possibly <= 0) of 16 consecutive gradient values, times f
 template <typename T>
 __device__ __forceinline__ void store16(T* dst, const uint32_t (&r)[16], float f, int n) {
@@ -194,6 +197,8 @@ __device__ __forceinline__ void diff_dq_body(const CUtensorMap& tmap_q, const CU
     const float* st = prm.stats + (static_cast<int64_t>(bi) * p.heads + hi) * 4 * prm.n_pad + qi;   // q0 + 127 < n_pad
     const float nlse1 = st[0], nlse2 = st[prm.n_pad], nd1 = st[2 * prm.n_pad], nd2 = st[3 * prm.n_pad];
     const float nlam = -diff_lam(p, hi);
+    const float2 c2 = make_float2(c, c), nl1 = make_float2(nlse1, nlse1), nl2 = make_float2(nlse2, nlse2);
+    const float2 nd1_2 = make_float2(nd1, nd1), lam2 = make_float2(nlam, nlam), lam_nd2 = make_float2(nlam * nd2, nlam * nd2);
     const int lim = p.causal ? min(p.nk - 1, qi + shift) : p.nk - 1;   // last key of this row
     bool alive = true;
     for (int j = 0; j < n_t; ++j) {
@@ -208,20 +213,23 @@ __device__ __forceinline__ void diff_dq_body(const CUtensorMap& tmap_q, const CU
       const int kb = j * 64 + 16 * cq;
       const bool masked = j * 64 + 64 > p.nk || (p.causal && j * 64 + 63 > q0 + shift);
       uint32_t d1[8], d2[8];
+      // (pairs: fma.f32x2 and its kind; lam goes into the second map's G - D)
+      auto tile = [&](auto with_mask) {
 #pragma unroll
-      for (int i = 0; i < 16; i += 2) {
-        float a[2], b[2];
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const float gv = __uint_as_float(g[i + e]);
-          float x1 = fast_exp2(fmaf(__uint_as_float(s1[i + e]), c, nlse1)), x2 = fast_exp2(fmaf(__uint_as_float(s2[i + e]), c, nlse2));
-          if (masked && kb + i + e > lim) x1 = x2 = 0.f;
-          a[e] = x1 * (gv + nd1);
-          b[e] = (nlam * x2) * (gv + nd2);
+        for (int i = 0; i < 16; i += 2) {
+          const float2 gv = pair(g, i);
+          float2 x1 = exp2_pair(__ffma2_rn(pair(s1, i), c2, nl1)), x2 = exp2_pair(__ffma2_rn(pair(s2, i), c2, nl2));
+          if (decltype(with_mask)::value) {
+            if (kb + i > lim) x1.x = x2.x = 0.f;
+            if (kb + i + 1 > lim) x1.y = x2.y = 0.f;
+          }
+          const float2 a = __fmul2_rn(x1, __fadd2_rn(gv, nd1_2)), b = __fmul2_rn(x2, __ffma2_rn(gv, lam2, lam_nd2));
+          d1[i >> 1] = pack2<T>(a.x, a.y);
+          d2[i >> 1] = pack2<T>(b.x, b.y);
         }
-        d1[i >> 1] = pack2<T>(a[0], a[1]);
-        d2[i >> 1] = pack2<T>(b[0], b[1]);
-      }
+      };
+      if (masked) tile(std::true_type{});
+      else tile(std::false_type{});
       tmem_st8(t, d1);
       tmem_st8(t + 64, d2);
       tmem_wait_st();
@@ -402,26 +410,32 @@ __device__ __forceinline__ void diff_dkv_body(const CUtensorMap& tmap_q, const C
         const float4* vec = reinterpret_cast<const float4*>(smem_gen + vec_off + st * kVecBytes) + 4 * cq;
         const int qc = q_tile0 + 16 * cq;
         const bool masked = p.causal && q_tile0 + shift < k0 + 127;    // some query of the tile does not see some key
+        const float2 c2 = make_float2(c, c), lam2 = make_float2(nlam, nlam);
+        auto tile = [&](auto with_mask) {
 #pragma unroll
-        for (int i4 = 0; i4 < 4; ++i4) {
-          const float4 l1 = vec[i4], l2 = vec[16 + i4], e1 = vec[32 + i4], e2 = vec[48 + i4];
-          const float nl1[4] = {l1.x, l1.y, l1.z, l1.w}, nl2[4] = {l2.x, l2.y, l2.z, l2.w};
-          const float nd1[4] = {e1.x, e1.y, e1.z, e1.w}, nd2[4] = {e2.x, e2.y, e2.z, e2.w};
-          float pv[4], a[4], b[4];
+          for (int i4 = 0; i4 < 4; ++i4) {
+            const float4 l1 = vec[i4], l2 = vec[16 + i4], e1 = vec[32 + i4], e2 = vec[48 + i4];
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const int i = 4 * i4 + e;
-            const float gv = __uint_as_float(g[i]);
-            float x1 = fast_exp2(fmaf(__uint_as_float(s1[i]), c, nl1[e])), x2 = nlam * fast_exp2(fmaf(__uint_as_float(s2[i]), c, nl2[e]));
-            if (masked && key > qc + i + shift) x1 = x2 = 0.f;
-            pv[e] = x1 + x2;
-            a[e] = x1 * (gv + nd1[e]);
-            b[e] = x2 * (gv + nd2[e]);
+            for (int h = 0; h < 2; ++h) {
+              const int i = 4 * i4 + 2 * h;
+              const float2 nl1 = h ? make_float2(l1.z, l1.w) : make_float2(l1.x, l1.y), nl2 = h ? make_float2(l2.z, l2.w) : make_float2(l2.x, l2.y);
+              const float2 nd1 = h ? make_float2(e1.z, e1.w) : make_float2(e1.x, e1.y), nd2 = h ? make_float2(e2.z, e2.w) : make_float2(e2.x, e2.y);
+              const float2 gv = pair(g, i);
+              float2 x1 = exp2_pair(__ffma2_rn(pair(s1, i), c2, nl1)), x2 = exp2_pair(__ffma2_rn(pair(s2, i), c2, nl2));
+              if (decltype(with_mask)::value) {
+                if (key > qc + i + shift) x1.x = x2.x = 0.f;
+                if (key > qc + i + 1 + shift) x1.y = x2.y = 0.f;
+              }
+              x2 = __fmul2_rn(x2, lam2);
+              const float2 pv = __fadd2_rn(x1, x2), a = __fmul2_rn(x1, __fadd2_rn(gv, nd1)), b = __fmul2_rn(x2, __fadd2_rn(gv, nd2));
+              pk[i >> 1] = pack2<T>(pv.x, pv.y);
+              d1[i >> 1] = pack2<T>(a.x, a.y);
+              d2[i >> 1] = pack2<T>(b.x, b.y);
+            }
           }
-          pk[2 * i4] = pack2<T>(pv[0], pv[1]); pk[2 * i4 + 1] = pack2<T>(pv[2], pv[3]);
-          d1[2 * i4] = pack2<T>(a[0], a[1]); d1[2 * i4 + 1] = pack2<T>(a[2], a[3]);
-          d2[2 * i4] = pack2<T>(b[0], b[1]); d2[2 * i4 + 1] = pack2<T>(b[2], b[3]);
-        }
+        };
+        if (masked) tile(std::true_type{});
+        else tile(std::false_type{});
       }
       if (it > 0) {
         // the products of the tile before have read what is overwritten now
