@@ -469,6 +469,20 @@ merge_kernel(const DecodeParams p, int n_parts) {
   auto written = [&](int part) { return !(part >= from[0] && part < to[0]) && !(part >= from[1] && part < to[1]); };
   const int64_t step = static_cast<int64_t>(p.kv_heads) * rows * MAPS;      // from one part to the next
   const int64_t first = (static_cast<int64_t>(g) * rows + row) * MAPS;
+  // eight parts' sums on their way (of parts that were not written too: whatever stands there is not used)
+  auto load8 = [&](float (&x)[kAhead][4], const float* ps, int p0) {
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) {
+      const float* src = ps + min(p0 + u, n_parts - 1) * step * p.v_dim;
+      if (VEC == 4) {
+        const float4 v = lane * 4 < p.v_dim ? *reinterpret_cast<const float4*>(src) : make_float4(0.f, 0.f, 0.f, 0.f);
+        x[u][0] = v.x; x[u][1] = v.y; x[u][2] = v.z; x[u][3] = v.w;
+      } else {
+#pragma unroll
+        for (int e = 0; e < kCols; ++e) x[u][e] = lane + 32 * e < p.v_dim ? src[32 * e] : 0.f;
+      }
+    }
+  };
   float total[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
   for (int m = 0; m < MAPS; ++m) {
@@ -477,6 +491,8 @@ merge_kernel(const DecodeParams p, int n_parts) {
     const float* ps = p.s + (first + m) * p.v_dim + lane * VEC;
     float top = -CUDART_INF_F, zs = 0.f, acc[4] = {0.f, 0.f, 0.f, 0.f};
     for (int p0 = 0; p0 < n_parts; p0 += 32) {
+      float x[kAhead][4];
+      load8(x, ps, p0);                                 // (beside the weights: one latency less)
       float m_part = -CUDART_INF_F, z_part = 0.f;
       if (p0 + lane < n_parts && written(p0 + lane)) {
         m_part = pm[(p0 + lane) * step];
@@ -484,7 +500,7 @@ merge_kernel(const DecodeParams p, int n_parts) {
       }
       float best = m_part;
 #pragma unroll
-      for (int x = 16; x > 0; x >>= 1) best = fmaxf(best, __shfl_xor_sync(0xffffffffu, best, x));
+      for (int y = 16; y > 0; y >>= 1) best = fmaxf(best, __shfl_xor_sync(0xffffffffu, best, y));
       if (best > top) {                                 // (more than 32 parts: what came before is rescaled)
         const float alpha = exp2f(top - best);
         zs *= alpha;
@@ -496,24 +512,12 @@ merge_kernel(const DecodeParams p, int n_parts) {
       zs += z_part != 0.f ? f * z_part : 0.f;
       const int n = min(32, n_parts - p0);
       for (int j0 = 0; j0 < n; j0 += kAhead) {
-        float x[kAhead][4];
+        if (j0 > 0) load8(x, ps, p0 + j0);
 #pragma unroll
         for (int u = 0; u < kAhead; ++u) {
-          const bool take = __shfl_sync(0xffffffffu, f, j0 + u) != 0.f;       // (lanes beyond n have f = 0)
-          const float* src = ps + (p0 + j0 + u) * step * p.v_dim;
-          if (VEC == 4) {
-            const float4 v = take && lane * 4 < p.v_dim ? *reinterpret_cast<const float4*>(src) : make_float4(0.f, 0.f, 0.f, 0.f);
-            x[u][0] = v.x; x[u][1] = v.y; x[u][2] = v.z; x[u][3] = v.w;
-          } else {
+          const float fj = __shfl_sync(0xffffffffu, f, j0 + u);               // (lanes beyond n have f = 0)
 #pragma unroll
-            for (int e = 0; e < kCols; ++e) x[u][e] = take && lane + 32 * e < p.v_dim ? src[32 * e] : 0.f;
-          }
-        }
-#pragma unroll
-        for (int u = 0; u < kAhead; ++u) {
-          const float fj = __shfl_sync(0xffffffffu, f, j0 + u);
-#pragma unroll
-          for (int e = 0; e < 4; ++e) acc[e] = fmaf(fj, x[u][e], acc[e]);
+          for (int e = 0; e < 4; ++e) acc[e] = fj != 0.f ? fmaf(fj, x[u][e], acc[e]) : acc[e];
         }
       }
     }
