@@ -7,13 +7,14 @@ attention over a shared prefix, differential attention) have no counterpart in t
 from .attention import twopass_attention
 from .attention_bwd import twopass_attention_backward, twopass_attention_train, twopass_attention_with_state
 from .differential import differential_attention, differential_attention_train, differential_lambda
-from .rotary import rotary_embedding, rotary_frequencies
+from .rotary import Rotary, rotary_embedding, rotary_frequencies
 from .shared_prefix import shared_prefix_attention
 from .timm_dropin import PatchReport, patch_timm_attention
 from .timm_dropin_bwd import TrainPatchReport, patch_timm_attention_train
 
 __all__ = [
     "PatchReport",
+    "Rotary",
     "TrainPatchReport",
     "differential_attention",
     "differential_attention_train",

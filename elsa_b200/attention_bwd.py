@@ -15,6 +15,7 @@ from typing import Literal, Optional
 import torch
 
 from . import _lib
+from .rotary import Rotary
 from .attention import (_DeviceScope, _aligned, _bhnd_strides, _cached_bytes, _canonical_bias, _check_qkv, _empty_like_layout, _forward_impl, _i64x,
                         _in_place_or_copy, _resolve_common, _resolve_keywords, _validate_warps)
 
@@ -426,13 +427,21 @@ class _PackedQkvAttentionAutograd(torch.autograd.Function):
 
 
 def twopass_attention_qkvpacked(qkv: torch.Tensor, *, bias: Optional[torch.Tensor] = None, is_causal: bool = False,
-                                train: bool = True, **fwd_kwargs) -> torch.Tensor:
+                                train: bool = True, rotary: Optional[Rotary] = None, **fwd_kwargs) -> torch.Tensor:
     """Attention on a packed qkv [B, N, 3, H, D] (not an entry point of the reference: the form its hooks would need to
     avoid their per-layer copies, src/elsa_twopass_clean/timm_dropin.py:46-55, timm_dropin_bwd.py:68-73).
     Returns out as a [B, H, N, D] view of [B, N, H, D] memory, so `out.transpose(1, 2).reshape(B, N, H*D)` is free.
-    train=False skips autograd and the row state."""
+    train=False skips autograd and the row state.  `rotary` turns q and k by their positions first (one launch that reads them in place;
+    k, v are read in place after it as well)."""
     if qkv.dim() != 5 or qkv.shape[2] != 3:
         raise ValueError("qkv must have shape [B,N,3,H,D]")
+    if rotary is not None:
+        from .attention import twopass_attention
+        q, k, v = qkv.permute(2, 0, 3, 1, 4).unbind(0)
+        q, k = rotary.apply(q, k)
+        if not train:
+            fwd_kwargs = {name: val for name, val in fwd_kwargs.items() if not name.startswith("bwd_")}
+        return (twopass_attention_train if train else twopass_attention)(q, k, v, bias=bias, is_causal=is_causal, **fwd_kwargs)
     # the backward tile hints of twopass_attention_train are validated and advisory, as there
     if fwd_kwargs.get("bwd_input_precision", "auto") not in ("auto", "ieee", "tf32", "tf32x3"):
         raise ValueError("input_precision must be 'auto', 'ieee', 'tf32', or 'tf32x3'")

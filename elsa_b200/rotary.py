@@ -8,7 +8,7 @@ from __future__ import annotations
 import ctypes
 import functools
 import math
-from typing import Literal, Optional, Union
+from typing import Literal, NamedTuple, Optional, Union
 
 import torch
 
@@ -250,3 +250,16 @@ def rotary_embedding(
         torch.autograd.graph.increment_version((q,) if k is None else (q, k))     # (what a graph had saved is gone)
         return q if k is None else (q, k)
     return _RotaryAutograd.apply(q, k, frequencies, positions, magnitude, bool(interleaved))
+
+
+class Rotary(NamedTuple):
+    """Rotary positions as one value, for calls that apply them on the way: `twopass_attention_qkvpacked(..., rotary=Rotary(...))` and the
+    ViT hooks (`patch_timm_attention(model, elsa_kwargs={"rotary": Rotary(...)})`).  The fields are `rotary_embedding`'s arguments."""
+
+    frequencies: torch.Tensor
+    positions: Optional[torch.Tensor] = None
+    interleaved: bool = False
+    magnitude: float = 1.0
+
+    def apply(self, q: torch.Tensor, k: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
+        return rotary_embedding(q, k, self.frequencies, positions=self.positions, interleaved=self.interleaved, magnitude=self.magnitude)

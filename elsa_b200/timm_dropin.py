@@ -84,8 +84,12 @@ class _VitAttentionBase(nn.Module):
         else:
             q, k, v = _split_heads(qkv, (batch, seq_len), self.num_heads, self.head_dim)
             q, k = self.q_norm(q), self.k_norm(k)
+            kwargs = self._op_kwargs(seq_len, q.dtype)
+            rotary = kwargs.pop("rotary", None)
+            if rotary is not None:
+                q, k = rotary.apply(q, k)
             op: Callable = twopass_attention_train if self._training_op else twopass_attention
-            y = op(q, k, v, **self._op_kwargs(seq_len, q.dtype))
+            y = op(q, k, v, **kwargs)
         y = y.transpose(1, 2).reshape(batch, seq_len, self.attn_dim)
         return self.proj_drop(self.proj(self.norm(y)))
 
@@ -107,6 +111,8 @@ class _SwinWindowAttentionBase(nn.Module):
         self.relative_position_bias_table = nn.Parameter(source.relative_position_bias_table.detach().clone())
         self.register_buffer("relative_position_index", source.relative_position_index.detach().clone(),
                              persistent=False)
+        if (elsa_kwargs or {}).get("rotary") is not None:
+            raise ValueError("rotary positions are for ViT attention; a Swin window has its relative-position bias")
         self.elsa_kwargs = dict(elsa_kwargs or {})
 
     def _get_rel_pos_bias(self) -> torch.Tensor:
