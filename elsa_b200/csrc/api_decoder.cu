@@ -231,7 +231,7 @@ extern "C" int elsa_differential_forward(const void* q, const void* k, const voi
 extern "C" int64_t elsa_differential_backward_workspace_bytes(int dtype, int batch, int heads, int kv_heads, int nq, int nk, int head_dim,
                                                               int v_dim) {
   DiffPlan pl;
-  return plan_diff(dtype, batch, heads, kv_heads, nq, nk, head_dim, v_dim, &pl) == ELSA_OK ? diff_stats_bytes(batch, heads, nq) : -1;
+  return plan_diff(dtype, batch, heads, kv_heads, nq, nk, head_dim, v_dim, &pl) == ELSA_OK ? diff_stats_bytes(batch, heads, nq) + diff_dlam_bytes(batch, heads, nq) : -1;
 }
 
 extern "C" int elsa_differential_backward(const void* q, const void* k, const void* v, const void* lam, int lam_dtype, int lam_stride,
@@ -245,7 +245,9 @@ extern "C" int elsa_differential_backward(const void* q, const void* k, const vo
   if (!q || !lam || !out || !out2 || !lse || !dout || !dq || !strides || (nk > 0 && (!k || !v || !dk || !dv)) || !dtype_ok(lam_dtype) || !(scale > 0.0))
     return ELSA_ERR_INVALID_ARGUMENT;
   if (batch > 32767) return ELSA_ERR_UNSUPPORTED;
-  if (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 255u) || workspace_bytes < diff_stats_bytes(batch, heads, nq)) return ELSA_ERR_WORKSPACE;
+  if (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 255u) || 
+      workspace_bytes < diff_stats_bytes(batch, heads, nq) + diff_dlam_bytes(batch, heads, nq))
+    return ELSA_ERR_WORKSPACE;
   auto st = static_cast<cudaStream_t>(stream);
   DiffParams d = diff_params(q, k, v, lam, lam_dtype, lam_stride, strides, batch, heads, kv_heads, nq, nk, head_dim, v_dim, is_causal, scale);
   auto at = [&](int i) { return Strides{strides[3 * i], strides[3 * i + 1], strides[3 * i + 2]}; };
@@ -253,11 +255,13 @@ extern "C" int elsa_differential_backward(const void* q, const void* k, const vo
   d.dout = dout; d.gs = at(4);
   d.dq = dq; d.dk = dk; d.dv = dv; d.dqs = at(5); d.dks = at(6); d.dvs = at(7);
   d.dlam = dlam;
+  d.dlam_parts = dlam ? reinterpret_cast<float*>(static_cast<char*>(workspace) + diff_stats_bytes(batch, heads, nq)) : nullptr;
   float* stats = static_cast<float*>(workspace);
   const bool tiles = diff_tc_sizes(dtype, head_dim, v_dim) && diff_inputs_in_tiles(d) && diff_rows_ok(dout, d.gs, v_dim, heads, batch) &&
                      diff_rows_ok(dq, d.dqs, head_dim, 2 * heads, batch) &&
                      (nk == 0 || (diff_rows_ok(dk, d.dks, head_dim, 2 * kv_heads, batch) && diff_rows_ok(dv, d.dvs, v_dim, kv_heads, batch)));
   if (tiles && (rc = device_status_ok()) != ELSA_OK) return rc;
   if ((rc = diff_stats(d, stats, dtype, st)) != ELSA_OK) return rc;
-  return tiles ? diff_bwd_tc(d, stats, dtype, st) : diff_bwd_any(d, stats, dtype, st);
+  if ((rc = tiles ? diff_bwd_tc(d, stats, dtype, st) : diff_bwd_any(d, stats, dtype, st)) != ELSA_OK || !dlam) return rc;
+  return diff_dlam(d, static_cast<int>(cdiv64(nq, tiles ? kDiffTcRows : kDiffAnyRows)), st);
 }

@@ -20,15 +20,20 @@ struct DiffParams {
   const void* dout; Strides gs;
   void* dq; void* dk; void* dv; Strides dqs, dks, dvs;
   void* dlam;                                    // like lam: a value for each head, or one (null: not wanted)
+  float* dlam_parts;                             // [B * heads][query tiles of the backward kernel]: sums of P2 G over a tile's rows and all keys
 };
 
 // sizes that the tcgen05 kernels take (16-bit types), and the strides and addresses that their tensor maps ask for
 bool diff_tc_sizes(int dtype, int head_dim, int v_dim);
 bool diff_rows_ok(const void* base, const Strides& s, int row, int heads, int batch);
-// row statistics of the backward, [B * heads][-LSE1, -LSE2, -D1, -D2][n_pad] with n_pad = nq rounded up to 128, and dlam (diff_any.cu)
-inline int64_t diff_stats_bytes(int batch, int heads, int nq) { return static_cast<int64_t>(batch) * heads * 4 * align_up(nq, 128) * 4; }
+// row statistics of the backward, [B * heads][-LSE1, -LSE2, -D1, -D2][n_pad] with n_pad = nq rounded up to 128 (diff_any.cu)
+inline int64_t diff_stats_bytes(int batch, int heads, int nq) { return align_up(static_cast<int64_t>(batch) * heads * 4 * align_up(nq, 128) * 4, 256); }
 int diff_stats(const DiffParams& p, float* stats, int dtype, cudaStream_t st);
+// the most parts that a backward kernel leaves, and their sum, once it has run: dlam[h] = -(sum over the batch and the tiles)
+inline int64_t diff_dlam_bytes(int batch, int heads, int nq) { return align_up(static_cast<int64_t>(batch) * heads * cdiv64(nq, 32) * 4, 256); }
+int diff_dlam(const DiffParams& p, int tiles, cudaStream_t st);
 // dq, dk, dv from them: of any type (diff_any.cu), 16-bit in tiles (diff_bwd_tc.cu)
+constexpr int kDiffAnyRows = 32, kDiffTcRows = 128;    // query rows of one of dlam's parts
 int diff_bwd_any(const DiffParams& p, const float* stats, int dtype, cudaStream_t st);
 int diff_bwd_tc(const DiffParams& p, const float* stats, int dtype, cudaStream_t st);
 

@@ -3,10 +3,11 @@
 //
 // With G = g V^T (g the gradient of out, shared by both maps) and D_m = g . (P_m V), row by row,
 //     dS1 = P1 (G - D1),  dS2 = -lam P2 (G - D2)          dQ_m = scale dS_m K_m,  dK_m = scale dS_m^T Q_m
-//     dV = (P1 - lam P2)^T g                              dlam = -sum of D2 over the head's rows
+//     dV = (P1 - lam P2)^T g                              dlam = -sum over rows and keys of P2 G
 // P is recomputed from the scores and each row's log2 sum, P = 2^(S scale log2 e - LSE).  D2 = g . out2 with out2 = P2 V from the
-// forward, and D1 = g . out + lam D2, since out = P1 V - lam P2 V.  Gradients of shared key heads are summed in the kernels that own
-// them, in a fixed order: no atomics anywhere.
+// forward, and D1 = g . out + lam D2, since out = P1 V - lam P2 V.  dlam is the sum of D2 too, of terms of either sign that may cancel to
+// next to nothing, while the D2 of a 16-bit out2 is known to 2^-9 only: it is summed from P2 and G in fp32, as the dQ kernels have them.
+// Gradients of shared key heads are summed in the kernels that own them, in a fixed order: no atomics anywhere.
 //
 // The kernels of any type work in fp32 on split tf32 operands (tf32.cuh): a block of eight warps owns 32 rows and streams 64 of the
 // other side at a time, a warp has a 16 x 16 block of S1, S2 and G in its accumulators, turns them into dS1, dS2 (and P1 - lam P2)
@@ -20,7 +21,7 @@ namespace elsa {
 
 namespace {
 
-constexpr int kThreads = 256, kOwn = 32, kStream = 64, kValue = 128;   // rows a block owns, rows of a streamed tile, most value columns
+constexpr int kThreads = 256, kOwn = kDiffAnyRows, kStream = 64, kValue = 128;   // rows a block owns, rows of a streamed tile, most value columns
 
 // stats: [B * heads][-LSE1, -LSE2, -D1, -D2][n_pad]; padding rows hold -inf, -inf, 0, 0.  A warp takes eight consecutive rows, two at a
 // time with 16 lanes each: all its loads (16 bytes, where rows allow that) are in flight at once and each statistic of the eight rows
@@ -100,16 +101,16 @@ diff_stats_kernel(const DiffParams p, float* __restrict__ stats, int n_pad) {
   }
 }
 
-// dlam[h] = sum of -D2 over the batch and the rows (padding is 0): a block per head, or one for all heads where lam is one value
-__global__ void __launch_bounds__(512)
-diff_dlam_kernel(const float* __restrict__ stats, void* dlam, int dlam_dtype, int batch, int heads, int n_pad, int all) {
-  __shared__ float part[16];
+// dlam[h] = -(sum of its parts): a block per head, or one for all heads where lam is one value
+__global__ void __launch_bounds__(256)
+diff_dlam_kernel(const float* __restrict__ parts, void* dlam, int dlam_dtype, int batch, int heads, int tiles, int all) {
+  __shared__ float part[8];
   const int h0 = all ? 0 : blockIdx.x, h1 = all ? heads : h0 + 1;
   float sum = 0.f;
   for (int b = 0; b < batch; ++b)
     for (int h = h0; h < h1; ++h) {
-      const float* src = stats + ((static_cast<int64_t>(b) * heads + h) * 4 + 3) * n_pad;
-      for (int r = threadIdx.x; r < n_pad; r += 512) sum += src[r];
+      const float* src = parts + (static_cast<int64_t>(b) * heads + h) * tiles;
+      for (int i = threadIdx.x; i < tiles; i += 256) sum += src[i];
     }
 #pragma unroll
   for (int x = 16; x > 0; x >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, x);
@@ -117,10 +118,10 @@ diff_dlam_kernel(const float* __restrict__ stats, void* dlam, int dlam_dtype, in
   __syncthreads();
   if (threadIdx.x == 0) {
     sum = 0.f;
-    for (int w = 0; w < 16; ++w) sum += part[w];
-    if (dlam_dtype == ELSA_F32) static_cast<float*>(dlam)[h0] = sum;
-    else if (dlam_dtype == ELSA_F16) static_cast<__half*>(dlam)[h0] = from_f32<__half>(sum);
-    else static_cast<__nv_bfloat16*>(dlam)[h0] = from_f32<__nv_bfloat16>(sum);
+    for (int w = 0; w < 8; ++w) sum += part[w];
+    if (dlam_dtype == ELSA_F32) static_cast<float*>(dlam)[h0] = -sum;
+    else if (dlam_dtype == ELSA_F16) static_cast<__half*>(dlam)[h0] = from_f32<__half>(-sum);
+    else static_cast<__nv_bfloat16*>(dlam)[h0] = from_f32<__nv_bfloat16>(-sum);
   }
 }
 
@@ -233,7 +234,7 @@ diff_dq_any_kernel(const DiffParams p, const float* __restrict__ stats, int n_pa
     nlse[0][j] = st[0]; nlse[1][j] = st[n_pad]; nd[0][j] = st[2 * n_pad]; nd[1][j] = st[3 * n_pad];
     lim[j] = p.causal ? min(p.nk - 1, row + 8 * j + shift) : p.nk - 1;
   }
-  float dq[2][DP / 8][4] = {};
+  float dq[2][DP / 8][4] = {}, dl = 0.f;
   const int end = p.causal ? min(p.nk, min(q0 + kOwn, p.nq) + shift) : p.nk;
   for (int k0 = 0; k0 < end; k0 += kStream) {
     __syncthreads();
@@ -254,11 +255,24 @@ diff_dq_any_kernel(const DiffParams p, const float* __restrict__ stats, int n_pa
 #pragma unroll
         for (int m = 0; m < 2; ++m) {
           const float x = seen ? exp2f(fmaf(s[m][n][e], p.scale_log2, nlse[m][j])) : 0.f;
+          if (m == 1) dl = fmaf(x, gv[n][e], dl);
           s[m][n][e] = x * (gv[n][e] + nd[m][j]) * (m ? -lam : 1.f);
         }
       }
 #pragma unroll
     for (int m = 0; m < 2; ++m) accumulate(dq[m], s[m], sk + m * kStream * kPitch + 16 * part * kPitch, kPitch, d8, lane);
+  }
+  if (p.dlam_parts) {
+#pragma unroll
+    for (int x = 16; x > 0; x >>= 1) dl += __shfl_xor_sync(0xffffffffu, dl, x);
+    __shared__ float part_of[kThreads / 32];
+    if (lane == 0) part_of[warp] = dl;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+      dl = 0.f;
+      for (int x = 0; x < kThreads / 32; ++x) dl += part_of[x];
+      p.dlam_parts[(static_cast<int64_t>(b) * p.heads + h) * gridDim.x + q0 / kOwn] = dl;
+    }
   }
 #pragma unroll
   for (int m = 0; m < 2; ++m)
@@ -360,10 +374,12 @@ int diff_stats(const DiffParams& p, float* stats, int dtype, cudaStream_t st) {
   else if (dtype == ELSA_F16) diff_stats_kernel<__half><<<grid, 256, 0, st>>>(p, stats, n_pad);
   else diff_stats_kernel<__nv_bfloat16><<<grid, 256, 0, st>>>(p, stats, n_pad);
   ELSA_LAUNCH_CHECK();
-  if (p.dlam) {
-    diff_dlam_kernel<<<p.lam_stride == 0 ? 1 : p.heads, 512, 0, st>>>(stats, p.dlam, p.lam_dtype, p.batch, p.heads, n_pad, p.lam_stride == 0);
-    ELSA_LAUNCH_CHECK();
-  }
+  return ELSA_OK;
+}
+
+int diff_dlam(const DiffParams& p, int tiles, cudaStream_t st) {
+  diff_dlam_kernel<<<p.lam_stride == 0 ? 1 : p.heads, 256, 0, st>>>(p.dlam_parts, p.dlam, p.lam_dtype, p.batch, p.heads, tiles, p.lam_stride == 0);
+  ELSA_LAUNCH_CHECK();
   return ELSA_OK;
 }
 

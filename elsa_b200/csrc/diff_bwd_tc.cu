@@ -83,6 +83,7 @@ __device__ __forceinline__ void diff_dq_body(const CUtensorMap& tmap_q, const CU
                                              const BwdParams2& prm, int bi) {
   extern __shared__ uint8_t smem_raw[];
   __shared__ __align__(8) uint64_t bars[2 * kStages + 6];
+  __shared__ float dlam_part[kFoldWarps];
   __shared__ uint32_t tmem_base_slot;
   __shared__ int abort_flag;
 
@@ -200,6 +201,7 @@ __device__ __forceinline__ void diff_dq_body(const CUtensorMap& tmap_q, const CU
     const float2 c2 = make_float2(c, c), nl1 = make_float2(nlse1, nlse1), nl2 = make_float2(nlse2, nlse2);
     const float2 nd1_2 = make_float2(nd1, nd1), lam2 = make_float2(nlam, nlam), lam_nd2 = make_float2(nlam * nd2, nlam * nd2);
     const int lim = p.causal ? min(p.nk - 1, qi + shift) : p.nk - 1;   // last key of this row
+    float2 dl[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};     // sum of P2 G: dlam's part of these rows
     bool alive = true;
     for (int j = 0; j < n_t; ++j) {
       if (!mbar_wait_warp(bar_sg(j & 1), (j >> 1) & 1, &abort_flag, prm.status, BAR_SG)) { alive = false; break; }
@@ -224,6 +226,7 @@ __device__ __forceinline__ void diff_dq_body(const CUtensorMap& tmap_q, const CU
             if (kb + i + 1 > lim) x1.y = x2.y = 0.f;
           }
           const float2 a = __fmul2_rn(x1, __fadd2_rn(gv, nd1_2)), b = __fmul2_rn(x2, __ffma2_rn(gv, lam2, lam_nd2));
+          dl[i >> 1 & 1] = __ffma2_rn(x2, gv, dl[i >> 1 & 1]);
           d1[i >> 1] = pack2<T>(a.x, a.y);
           d2[i >> 1] = pack2<T>(b.x, b.y);
         }
@@ -235,6 +238,18 @@ __device__ __forceinline__ void diff_dq_body(const CUtensorMap& tmap_q, const CU
       tmem_wait_st();
       tc_fence_before();
       mbar_arrive_warp(bar_ds(j & 1), lane);
+    }
+    if (p.dlam_parts) {
+      float sum = (dl[0].x + dl[0].y) + (dl[1].x + dl[1].y);
+#pragma unroll
+      for (int x = 16; x > 0; x >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, x);
+      if (lane == 0) dlam_part[warp] = sum;
+      named_barrier_sync(1, kFoldThreads);
+      if (warp == 0 && lane == 0) {
+        sum = 0.f;
+        for (int x = 0; x < kFoldWarps; ++x) sum += dlam_part[x];
+        p.dlam_parts[(static_cast<int64_t>(bi) * p.heads + hi) * n_qt + q0 / 128] = sum;
+      }
     }
     uint32_t r[2][16];
 #pragma unroll

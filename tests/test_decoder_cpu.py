@@ -157,7 +157,7 @@ def test_differential_backward_refuses_before_any_launch(lib):
     with pytest.raises(ValueError, match="CUDA"):
         E.differential_attention_train(q, k, v, 0.5)
     size = lib.elsa_differential_backward_workspace_bytes
-    assert size(1, 2, 4, 2, 3, 100, 64, 128) == 2 * 4 * 4 * 128 * 4 and size(1, 2, 4, 2, 3, 100, 64, 130) == -1
+    assert size(1, 2, 4, 2, 3, 100, 64, 128) >= 2 * 4 * (4 * 128 + 1) * 4 and size(1, 2, 4, 2, 3, 100, 64, 130) == -1
     st = (ctypes.c_int64 * 24)(*([64] * 24))
 
     def call(strides=st, ws=256, nbytes=1 << 40, dtype=1, lam_dtype=0, scale=0.125, **null):

@@ -251,7 +251,8 @@ def _gradients(q, k, v, lam, dout, causal, scale=None):
             grads[2][i, g] += pc.T @ go
             limits[2][i, g] += (e_pc + (h // hkv) * terms * pc.abs()).T @ go.abs()
             grads[3][j] -= dd[1].sum()
-            limits[3][j] += e_d2.sum() + (b * nq + 64) * u * dd[1].abs().sum()
+            # dlam is summed from P2 and G in fp32, not from the rounded outputs: the weight's error, G's, and the additions
+            limits[3][j] += (maps[1].p * (maps[1].e * gv.abs() + e_gv)).sum() + (nk + 600) * u * (maps[1].p * gv.abs()).sum()
     for t, lim in zip(grads, limits):
         lim += half * t.abs() * 1.01 + 2.0 ** -25
     return grads, limits
