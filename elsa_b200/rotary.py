@@ -96,6 +96,34 @@ def _overlaps(t: torch.Tensor) -> bool:
     return False
 
 
+def _meet(q: torch.Tensor, k: torch.Tensor) -> bool:
+    """Whether an element of q and one of k share memory, for two [B, H, N, D] views without overlaps of their own (`_overlaps`).  Views
+    of one buffer with the same strides, as of a packed projection, are told apart exactly; others count as meeting where the
+    ranges of their addresses do."""
+    size = q.element_size()
+    extent = lambda t: (sum((n - 1) * st for n, st in zip(t.shape[:3], t.stride()[:3])) + int(t.shape[3])) * size
+    offset = k.data_ptr() - q.data_ptr()
+    if offset >= extent(q) or -offset >= extent(k):
+        return False
+    axes = [(1, 1 - int(k.shape[3]), int(q.shape[3]) - 1)]               # (stride, least and most that an index of q is ahead of k's)
+    for sq, sk, nq, nk in zip(q.stride()[:3], k.stride()[:3], q.shape[:3], k.shape[:3]):
+        if nq > 1 and nk > 1 and sq != sk:
+            return True
+        if nq > 1 or nk > 1:
+            axes.append((sq if nq > 1 else sk, 1 - nk, nq - 1))
+    axes.sort(reverse=True)
+
+    def reaches(rest, axes):
+        if not axes:
+            return rest == 0
+        (stride, low, high), below = axes[0], axes[1:]
+        least, most = (sum(x[0] * x[i] for x in below) for i in (1, 2))
+        first, last = max(low, -((most - rest) // stride)), min(high, (rest - least) // stride)
+        return any(reaches(rest - e * stride, below) for e in range(first, last + 1))
+
+    return offset % size != 0 or reaches(offset // size, axes)
+
+
 def _launch(q, k, q_out, k_out, frequencies, positions, magnitude, interleaved, inverse):
     b, h, n, d = q.shape
     args_k = (None, None, None, 0)
@@ -244,7 +272,7 @@ def rotary_embedding(
         for t in (q,) if k is None else (q, k):
             if _row_strides(t) is None or _overlaps(t):
                 raise ValueError("inplace=True needs rows of contiguous elements that do not overlap")
-        if k is not None and q.numel() > 0 and q.data_ptr() == k.data_ptr():
+        if k is not None and q.numel() > 0 and k.numel() > 0 and _meet(q, k):
             raise ValueError("inplace=True needs q and k in different memory")
         _rotate(q, k, frequencies, positions, magnitude, interleaved, inplace=True)
         torch.autograd.graph.increment_version((q,) if k is None else (q, k))     # (what a graph had saved is gone)

@@ -70,6 +70,40 @@ def test_rotary_overlap_check():
     assert not _overlaps(base[:1, :1, :1])
 
 
+def _elements(t):
+    at = t.storage_offset()
+    return {at + b * t.stride(0) + h * t.stride(1) + n * t.stride(2) + d for b in range(t.shape[0]) for h in range(t.shape[1])
+            for n in range(t.shape[2]) for d in range(t.shape[3])}
+
+
+@pytest.mark.parametrize("seed", range(8))
+def test_rotary_in_place_tells_views_that_share_elements(seed):
+    from elsa_b200 import rotary
+    gen = torch.Generator().manual_seed(seed)
+    pick = lambda n: int(torch.randint(n, (), generator=gen))
+    found = {False: 0, True: 0}
+    for _ in range(200):
+        b, n, width, d = 1 + pick(3), 1 + pick(4), 4 + pick(3), 2 * (1 + pick(3))
+        pool = torch.zeros(b * n * width * d + 16)
+        x = pool[:b * n * width * d].view(b, n, width * d)
+        if pick(4) == 0:                    # heads in front of tokens
+            x = pool[:b * n * width * d].view(b, width, n * d)
+            views = [x.view(b, width, n, d)] * 2
+        else:
+            shift = pick(2) * pick(d)       # half of a head's columns, or whole ones
+            views = [x[:, :, :(width - 1) * d].view(b, n, width - 1, d).transpose(1, 2),
+                     x[:, :, shift:shift + (width - 1) * d].unflatten(2, (width - 1, d)).transpose(1, 2)]
+        total = views[0].shape[1]
+        q, k = (v[:, (at := pick(total)):at + 1 + pick(total - at)] for v in views)
+        want = bool(_elements(q) & _elements(k))
+        found[want] += 1
+        assert rotary._meet(q, k) == want
+        assert rotary._meet(k, q) == want
+    assert min(found.values()) > 20
+    q = torch.zeros(1, 2, 4, 8)
+    assert rotary._meet(q, q.transpose(1, 2)) and not rotary._meet(q, torch.zeros(1, 2, 4, 8))
+
+
 def test_rotary_abi_refuses_before_any_launch(lib):
     import ctypes
     st = (ctypes.c_int64 * 6)(512, 256, 64, 512, 256, 64)

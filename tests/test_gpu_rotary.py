@@ -191,3 +191,18 @@ def test_another_stream_and_a_captured_call():
     graph.replay()
     again = E.rotary_embedding(q, k, f, positions=pos)
     assert torch.equal(out[0], again[0]) and torch.equal(out[1], again[1])
+
+
+def test_in_place_refuses_q_and_k_that_share_elements():
+    f = E.rotary_frequencies(16, device="cuda")[0]
+    pool = _inputs((2, 19, 6, 16), torch.float16, 31)
+    keep = pool.clone()
+    heads = pool.transpose(1, 2)
+    for q, k in ((heads[:, :4], heads[:, 3:]), (heads, heads), (heads[:, :4, :10], heads[:, 2:, 9:])):
+        q, k = q[:, :, :k.shape[2]], k[:, :, :q.shape[2]]
+        with pytest.raises(ValueError, match="different memory"):
+            E.rotary_embedding(q, k, f, inplace=True)
+    assert torch.equal(pool, keep)
+    want = E.rotary_embedding(heads[:, :4], heads[:, 4:], f)
+    E.rotary_embedding(heads[:, :4], heads[:, 4:], f, inplace=True)
+    assert torch.equal(heads, torch.cat(want, 1))
