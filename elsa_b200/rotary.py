@@ -233,7 +233,7 @@ def rotary_embedding(
     elements are read in place: views of a packed projection need no copy).  frequencies: [R / 2], fp64, from
     `rotary_frequencies`, with its `magnitude`.  positions: int32 or int64, [N] or [B, N], any values; None: 0 .. N-1.
     Dimension i is paired with i + R/2, or, with `interleaved`, 2i with 2i + 1; dimensions from R on stay as they are.
-    Differentiable in q and k.  `inplace` writes over q and k instead (no gradients then).  Returns q', or (q', k')."""
+    Differentiable in q and k (not in frequencies).  `inplace` writes over q and k instead (no gradients then).  Returns q', or (q', k')."""
     if not inplace and isinstance(q, torch.Tensor) and q.is_cuda:
         host = _lib.host()
         if host is not None:
@@ -263,6 +263,8 @@ def rotary_embedding(
             raise ValueError("positions must be int32 or int64 on the device of q")
         if positions.dim() not in (1, 2) or positions.shape[-1] != q.shape[2] or (positions.dim() == 2 and positions.shape[0] not in (1, q.shape[0])):
             raise ValueError("positions must have shape [N] or [B,N]")
+    if torch.is_grad_enabled() and frequencies.requires_grad:
+        raise ValueError("frequencies have no gradient: detach them")
     if not frequencies.is_contiguous():
         frequencies = frequencies.contiguous()
     magnitude = float(magnitude)

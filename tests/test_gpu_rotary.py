@@ -206,3 +206,14 @@ def test_in_place_refuses_q_and_k_that_share_elements():
     want = E.rotary_embedding(heads[:, :4], heads[:, 4:], f)
     E.rotary_embedding(heads[:, :4], heads[:, 4:], f, inplace=True)
     assert torch.equal(heads, torch.cat(want, 1))
+
+
+def test_frequencies_that_ask_for_a_gradient_are_refused():
+    """They would get none: a call must not drop it in silence."""
+    q = _inputs((1, 2, 5, 16), torch.float32, 32)
+    f = E.rotary_frequencies(16, device="cuda")[0].requires_grad_(True)
+    with pytest.raises(ValueError, match="no gradient"):
+        E.rotary_embedding(q, None, f)
+    with torch.no_grad():
+        want = E.rotary_embedding(q, None, f)
+    assert torch.equal(E.rotary_embedding(q, None, f.detach()), want)
