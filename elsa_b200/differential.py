@@ -192,6 +192,7 @@ def differential_attention_train(
     scale = _positive_scale(scale, sizes[5])
     if any(x == 0 for x in (sizes[0], sizes[1], sizes[3], sizes[4], sizes[6])):
         # nothing to attend to: zeros that depend on nothing but shapes (and have zero gradients)
-        zero = q.sum() * 0 + k.sum() * 0 + v.sum() * 0
-        return torch.zeros((sizes[0], sizes[1], sizes[3], sizes[6]), device=q.device, dtype=q.dtype) + zero.to(q.dtype)
+        # (sums of no elements: a sum of all of q may be infinite, or NaN)
+        zero = sum(t.flatten()[:0].sum() for t in (q, k, v) + ((lam.to(q.dtype),) if isinstance(lam, torch.Tensor) else ()))
+        return torch.zeros((sizes[0], sizes[1], sizes[3], sizes[6]), device=q.device, dtype=q.dtype) + zero
     return _DifferentialAutograd.apply(q, k, v, lam, sizes, bool(is_causal), scale)

@@ -417,3 +417,15 @@ def test_training_step_on_another_stream_and_captured(dtype):
     torch.cuda.synchronize()
     fresh = step()
     assert all(torch.equal(a, b) for a, b in zip(held, fresh))
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.float32])
+def test_training_without_keys_is_zeros_whatever_q_holds(dtype):
+    q, k, v, lam = _inputs(2, 2, 1, 300, 0, 64, 128, dtype)
+    q.fill_(100.0)                                     # (the sum of q is infinite in fp16)
+    q[1, 0, 7, 3] = float("nan")
+    leaves = [t.detach().requires_grad_(True) for t in (q, k, v, lam)]
+    out = E.differential_attention_train(*leaves)
+    assert out.shape == (2, 2, 300, 128) and out.dtype == dtype and not bool(out.any())
+    grads = torch.autograd.grad(out, leaves, torch.ones_like(out))
+    assert all(g.shape == t.shape and not bool(g.any()) for g, t in zip(grads, leaves))
