@@ -259,7 +259,7 @@ bool diff_covers(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, 
       c->kv_heads == 0 || c->heads % c->kv_heads || c->d > 128 || c->dv > 128)
     return false;
   if (!plain(lam) || dtype_code(lam.scalar_type()) < 0 || lam.device() != q.device() || lam.dim() > 1 ||
-      (lam.dim() == 1 && lam.size(0) != 1 && lam.size(0) != c->heads) || (lam.dim() == 1 && lam.size(0) > 1 && lam.stride(0) < 1))
+      (lam.dim() == 1 && lam.size(0) != 1 && lam.size(0) != c->heads) || (lam.dim() == 1 && lam.size(0) > 1 && (lam.stride(0) < 1 || lam.stride(0) > kMostSize)))
     return false;
   if (c->scale == 0.0) c->scale = 1.0 / std::sqrt(static_cast<double>(c->d));      // (the default)
   return !modes_active();

@@ -12,7 +12,7 @@ import torch
 
 from . import _lib
 from .attention import _DeviceScope, _aligned, _cached_bytes, _in_place_or_copy
-from .rotary import _check_saved, _once_differentiable
+from .rotary import _MAX_SIZE, _check_saved, _check_sizes, _once_differentiable
 from .shared_prefix import _check_lengths, _positive_scale, _readable, _strides
 
 
@@ -37,6 +37,7 @@ def _check(q, k, v, lam, who: str):
         raise ValueError("q, k, v must agree in batch and head_dim, k and v in heads and keys")
     if kv_heads == 0 or heads % kv_heads:
         raise ValueError("the number of output heads must be a multiple of the number of value heads")
+    _check_sizes(q, k, v)
     if q.device.type != "cuda":
         raise ValueError(f"{who} currently requires CUDA tensors")
     if q.dtype not in (torch.float16, torch.bfloat16, torch.float32):
@@ -58,6 +59,8 @@ def _lam_args(lam, heads, like):
     if not isinstance(lam, torch.Tensor):
         lam = torch.full((), float(lam), device=like.device, dtype=torch.float32)
     lam = lam.detach()
+    if lam.dim() == 1 and lam.stride(0) > _MAX_SIZE:
+        lam = lam.contiguous()
     stride = int(lam.stride(0)) if lam.dim() == 1 and lam.shape[0] > 1 else 0
     return lam, lam.data_ptr(), _lib.dtype_code(lam.dtype), stride
 

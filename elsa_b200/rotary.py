@@ -17,6 +17,14 @@ from .attention import _DeviceScope, _empty_like_layout
 
 _MAX_ROTARY_DIM = 256
 _MAX_HEAD_DIM = 1024
+_MAX_SIZE = (1 << 30) - 1
+
+
+def _check_sizes(*tensors):
+    """No axis longer than the kernels' 32-bit indices count."""
+    for t in tensors:
+        if any(n > _MAX_SIZE for n in t.shape):
+            raise ValueError(f"an axis of more than {_MAX_SIZE} elements is not supported by the current kernels")
 
 
 def rotary_frequencies(
@@ -245,6 +253,7 @@ def rotary_embedding(
         raise ValueError("q, k must have shape [B,H,N,D]")
     if k is not None and (k.shape[0] != q.shape[0] or k.shape[2:] != q.shape[2:]):
         raise ValueError("q and k must agree in batch, tokens, and head_dim")
+    _check_sizes(q, *(() if k is None else (k,)))
     if q.device.type != "cuda":
         raise ValueError("rotary_embedding currently requires CUDA tensors")
     if q.dtype not in (torch.float16, torch.bfloat16, torch.float32):

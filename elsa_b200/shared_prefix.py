@@ -13,6 +13,7 @@ import torch
 
 from . import _lib
 from .attention import _DeviceScope, _cached_bytes, _empty_like_layout
+from .rotary import _check_sizes
 
 
 def _strides(t: torch.Tensor):
@@ -83,6 +84,7 @@ def shared_prefix_attention(
         raise ValueError("q, k, k_prefix must agree in batch, key heads, and head_dim")
     if kv_heads == 0 or heads % kv_heads:
         raise ValueError("the number of query heads must be a multiple of the number of key heads")
+    _check_sizes(q, k_prefix, k)
     if q.device.type != "cuda":
         raise ValueError("shared_prefix_attention currently requires CUDA tensors")
     if q.dtype not in (torch.float16, torch.bfloat16, torch.float32):

@@ -203,3 +203,17 @@ def test_differential_backward_refuses_before_any_launch(lib):
         assert call(**{name: 0}) == 1
     assert call(strides=None) == 1 and call(dtype=8) == 1 and call(lam_dtype=8) == 1 and call(scale=-1.0) == 1
     assert call(ws=None) == 4 and call(ws=64) == 4 and call(nbytes=64) == 4
+
+
+def test_axes_that_32_bits_do_not_count_are_refused():
+    """(expanded: no memory behind them)"""
+    long = lambda *shape: torch.zeros((1,) * len(shape)).expand(shape)
+    n = 2 ** 32 + 1
+    with pytest.raises(ValueError, match="an axis of more than"):
+        E.rotary_embedding(long(1, 1, n, 2), None, torch.ones(1, dtype=torch.float64))
+    with pytest.raises(ValueError, match="an axis of more than"):
+        E.shared_prefix_attention(long(1, 1, 1, 8), long(1, n, 8), long(1, n, 8), long(1, 1, 4, 8), long(1, 1, 4, 8))
+    for call in (E.differential_attention, E.differential_attention_train):
+        with pytest.raises(ValueError, match="an axis of more than"):
+            call(long(1, 2, 1, 8), long(1, 2, n, 8), long(1, 1, n, 8), 0.5)
+
