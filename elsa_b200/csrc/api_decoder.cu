@@ -1,6 +1,7 @@
 // C-ABI layer of the operators of decoder models (rotary positions, attention over a shared prefix, differential attention):
 // argument validation and host orchestration.  Stream-ordered like api.cu; nothing allocates device memory or synchronises.
 #include <algorithm>
+#include <cfloat>
 
 #include "decode.cuh"
 #include "diff.cuh"
@@ -14,6 +15,9 @@ namespace {
 bool inputs_ok(const void* p, int heads, int n, int head_dim, int batch, int dtype) {
   return p && heads > 0 && n > 0 && batch > 0 && head_dim > 0 && dtype_ok(dtype);
 }
+
+// positive and finite in fp32, with log2 e too (a scale that is zero there would make NaN of a masked score)
+bool scale_ok(double scale) { return scale >= static_cast<double>(FLT_MIN) && scale * 1.4426950408889634 <= static_cast<double>(FLT_MAX); }
 
 // a tensor-core kernel's wait that gave up is reported by every later call that would launch one (api.cu)
 int device_status_ok() {
@@ -153,7 +157,7 @@ extern "C" int elsa_shared_prefix_attention(const void* q, const void* k_prefix,
   PrefixPlan pl;
   int rc = plan_prefix(dtype, batch, heads, kv_heads, nq, head_dim, n_prefix, n_own, &pl);
   if (rc != ELSA_OK) return rc;
-  if (!q || !out || !strides || (n_prefix > 0 && (!k_prefix || !v_prefix)) || (n_own > 0 && (!k || !v)) || !(scale > 0.0)) return ELSA_ERR_INVALID_ARGUMENT;
+  if (!q || !out || !strides || (n_prefix > 0 && (!k_prefix || !v_prefix)) || (n_own > 0 && (!k || !v)) || !scale_ok(scale)) return ELSA_ERR_INVALID_ARGUMENT;
   if (pl.bytes() > 0 && (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 255u) || workspace_bytes < pl.bytes())) return ELSA_ERR_WORKSPACE;
   auto st = static_cast<cudaStream_t>(stream);
   char* ws = static_cast<char*>(workspace);
@@ -200,7 +204,7 @@ extern "C" int elsa_differential_forward(const void* q, const void* k, const voi
   DiffPlan pl;
   int rc = plan_diff(dtype, batch, heads, kv_heads, nq, nk, head_dim, v_dim, &pl);
   if (rc != ELSA_OK) return rc;
-  if (!q || !lam || !out || !strides || (nk > 0 && (!k || !v)) || !dtype_ok(lam_dtype) || !(scale > 0.0)) return ELSA_ERR_INVALID_ARGUMENT;
+  if (!q || !lam || !out || !strides || (nk > 0 && (!k || !v)) || !dtype_ok(lam_dtype) || !scale_ok(scale)) return ELSA_ERR_INVALID_ARGUMENT;
   if (pl.bytes() > 0 && (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 255u) || workspace_bytes < pl.bytes())) return ELSA_ERR_WORKSPACE;
   auto st = static_cast<cudaStream_t>(stream);
   DiffParams d = diff_params(q, k, v, lam, lam_dtype, lam_stride, strides, batch, heads, kv_heads, nq, nk, head_dim, v_dim, is_causal, scale);
@@ -242,7 +246,7 @@ extern "C" int elsa_differential_backward(const void* q, const void* k, const vo
   DiffPlan pl;
   int rc = plan_diff(dtype, batch, heads, kv_heads, nq, nk, head_dim, v_dim, &pl);
   if (rc != ELSA_OK) return rc;
-  if (!q || !lam || !out || !out2 || !lse || !dout || !dq || !strides || (nk > 0 && (!k || !v || !dk || !dv)) || !dtype_ok(lam_dtype) || !(scale > 0.0))
+  if (!q || !lam || !out || !out2 || !lse || !dout || !dq || !strides || (nk > 0 && (!k || !v || !dk || !dv)) || !dtype_ok(lam_dtype) || !scale_ok(scale))
     return ELSA_ERR_INVALID_ARGUMENT;
   if (batch > 32767) return ELSA_ERR_UNSUPPORTED;
   if (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 255u) || 

@@ -349,13 +349,13 @@ bool get_double(PyObject* o, double* x) {
   *x = PyFloat_AsDouble(o);
   return !(*x == -1.0 && PyErr_Occurred());
 }
-constexpr double kDefaultScale = 0.0;               // what None stands for; 0 itself is refused, like every number that is not positive and finite
+constexpr double kDefaultScale = 0.0;               // what None stands for; 0 itself is refused, like every number that is not positive and finite in fp32
 bool get_scale(PyObject* o, double* x, bool* refused) {
   *refused = false;
   *x = kDefaultScale;
   if (o == Py_None) return true;
   if (!get_double(o, x)) return false;
-  *refused = !(*x > 0.0 && std::isfinite(*x));
+  *refused = !(*x >= 0x1p-126 && *x <= 0x1p127);
   return true;
 }
 

@@ -41,8 +41,8 @@ def _check_lengths(lengths, batch, device):
 
 def _positive_scale(scale, dim):
     scale = max(1, int(dim)) ** -0.5 if scale is None else float(scale)
-    if not 0.0 < scale < float("inf"):
-        raise ValueError("scale must be positive and finite")
+    if not 2.0 ** -126 <= scale <= 2.0 ** 127:           # (the kernels hold scale log2 e in fp32)
+        raise ValueError("scale must be positive and finite in fp32")
     return scale
 
 

@@ -362,7 +362,7 @@ int elsa_rotary(const void* q, void* q_out, const int64_t* q_strides, int q_head
  * query head h reads kv head h / (heads / kv_heads).  lengths: 32-bit integers on the device, clamped to 0 .. n_own; NULL: n_own.
  * `strides` = element strides, in this order: q {b, h, r}, k_prefix {h, r}, v_prefix {h, r}, k {b, h, r}, v {b, h, r}, out {b, h, r}; the
  * elements of a row are contiguous.  head_dim <= 128.  16-bit inputs whose rows start on 16-byte boundaries run on the tensor
- * cores.  n_prefix or n_own may be 0 (then its pointers are not looked at).  scale > 0.
+ * cores.  n_prefix or n_own may be 0 (then its pointers are not looked at).  scale: positive and finite in fp32.
  * workspace (256-byte aligned): elsa_shared_prefix_workspace_bytes; -1 for sizes that the call would refuse. */
 int64_t elsa_shared_prefix_workspace_bytes(int dtype, int batch, int heads, int kv_heads, int nq, int head_dim, int n_prefix, int n_own);
 int elsa_shared_prefix_attention(const void* q, const void* k_prefix, const void* v_prefix, const void* k, const void* v, void* out,
@@ -378,7 +378,7 @@ int elsa_shared_prefix_attention(const void* q, const void* k_prefix, const void
  * <= 64 whose rows start on 16-byte boundaries run on the tensor cores.
  * `strides` = element strides {batch, head, row} of q, k, v, out; the elements of a row are contiguous.
  * out2, lse: NULL, or what elsa_differential_backward needs: P2 v as contiguous [batch, heads, nq, v_dim] in `dtype`, and log2 of each
- * row's sum of 2^score as [2][batch * heads * nq] fp32.  scale > 0.  workspace: elsa_differential_workspace_bytes, 256-byte aligned. */
+ * row's sum of 2^score as [2][batch * heads * nq] fp32.  scale: positive and finite in fp32.  workspace: elsa_differential_workspace_bytes, 256-byte aligned. */
 int64_t elsa_differential_workspace_bytes(int dtype, int batch, int heads, int kv_heads, int nq, int nk, int head_dim, int v_dim);
 int elsa_differential_forward(const void* q, const void* k, const void* v, const void* lam, int lam_dtype, int lam_stride,
                               const int* lengths, void* out, const int64_t* strides, void* out2, float* lse, void* workspace,

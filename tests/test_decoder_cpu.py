@@ -182,6 +182,7 @@ def test_differential_refuses_before_any_launch(lib):
     for name in ("q", "k", "v", "lam", "out", "strides"):
         assert call(**{name: None}) == 1
     assert call(lam_dtype=7) == 1 and call(dtype=7) == 1 and call(kv=3) == 1 and call(scale=0.0) == 1 and call(scale=float("nan")) == 1
+    assert call(scale=1e-46) == 1 and call(scale=float("inf")) == 1 and call(scale=3e38) == 1
     assert call(ws=None) == 4 and call(ws=100) == 4 and call(nbytes=100) == 4
 
 

@@ -429,3 +429,12 @@ def test_training_without_keys_is_zeros_whatever_q_holds(dtype):
     assert out.shape == (2, 2, 300, 128) and out.dtype == dtype and not bool(out.any())
     grads = torch.autograd.grad(out, leaves, torch.ones_like(out))
     assert all(g.shape == t.shape and not bool(g.any()) for g, t in zip(grads, leaves))
+
+
+@pytest.mark.parametrize("scale", [1e-46, 1e39, float("inf"), float("nan"), 0.0])
+def test_a_scale_that_fp32_does_not_hold_is_refused(scale):
+    """(one that is zero there would turn masked scores into NaN)"""
+    q, k, v, lam = _inputs(1, 2, 2, 150, 150, 64, 128, torch.float16)
+    for call in (E.differential_attention, E.differential_attention_train):
+        with pytest.raises(ValueError, match="scale"):
+            call(q, k, v, lam, is_causal=True, scale=scale)

@@ -216,3 +216,10 @@ def test_another_stream_and_two_captured_graphs(b):
     lengths.fill_(80)                                        # the next token's step: lengths live on the device
     one.replay()
     assert torch.equal(a, E.shared_prefix_attention(*args, lengths=lengths))
+
+
+@pytest.mark.parametrize("scale", [1e-46, 1e39, float("inf"), float("nan"), 0.0])
+def test_a_scale_that_fp32_does_not_hold_is_refused(scale):
+    """(one that is zero there would turn masked scores into NaN)"""
+    with pytest.raises(ValueError, match="scale"):
+        E.shared_prefix_attention(*_inputs(2, 4, 2, 2, 64, 90, 20, torch.float16), scale=scale)
