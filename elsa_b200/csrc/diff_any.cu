@@ -101,17 +101,20 @@ diff_stats_kernel(const DiffParams p, float* __restrict__ stats, int n_pad) {
   }
 }
 
-// dlam[h] = -(sum of its parts): a block per head, or one for all heads where lam is one value
+// dlam[h] = -(sum of its parts): a block per head, or one for all heads where lam is one value.  (One walk over all parts, not one for
+// each sequence and head: their loads are independent.)
 __global__ void __launch_bounds__(256)
 diff_dlam_kernel(const float* __restrict__ parts, void* dlam, int dlam_dtype, int batch, int heads, int tiles, int all) {
   __shared__ float part[8];
-  const int h0 = all ? 0 : blockIdx.x, h1 = all ? heads : h0 + 1;
-  float sum = 0.f;
-  for (int b = 0; b < batch; ++b)
-    for (int h = h0; h < h1; ++h) {
-      const float* src = parts + (static_cast<int64_t>(b) * heads + h) * tiles;
-      for (int i = threadIdx.x; i < tiles; i += 256) sum += src[i];
-    }
+  const int h0 = all ? 0 : blockIdx.x;
+  float sum = 0.f;                                       // (there are fewer than 2^30 parts)
+  if (all) {
+#pragma unroll 8
+    for (int i = threadIdx.x; i < batch * heads * tiles; i += 256) sum += parts[i];
+  } else {
+#pragma unroll 4
+    for (int i = threadIdx.x; i < batch * tiles; i += 256) sum += parts[(i / tiles * heads + h0) * tiles + i % tiles];
+  }
 #pragma unroll
   for (int x = 16; x > 0; x >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, x);
   if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = sum;
