@@ -98,7 +98,8 @@ int plan_diff(int dtype, int batch, int heads, int kv_heads, int nq, int nk, int
     return ELSA_ERR_INVALID_ARGUMENT;
   if (head_dim > 128 || v_dim > 128) return ELSA_ERR_UNSUPPORTED;
   const int64_t rows_b = static_cast<int64_t>(heads / kv_heads) * nq, rows = rows_b * batch;
-  if (rows * kv_heads > 0x1fffffff || heads > 65535 || batch > 65535 || nk > 0x3fffffff || nq > 0x3fffffff) return ELSA_ERR_UNSUPPORTED;
+  // (nq: the backward's four statistics of a head are indexed in 32 bits)
+  if (rows * kv_heads > 0x1fffffff || heads > 65535 || batch > 65535 || nk > 0x3fffffff || nq > 0xfffffff) return ELSA_ERR_UNSUPPORTED;
   pl->tensor_tiles = rows_b > kSplitRows && diff_tc_sizes(dtype, head_dim, v_dim);
   pl->split_width = nk > 0 ? split_width(static_cast<int64_t>(batch) * kv_heads * cdiv64(rows_b, 16), nk) : 1;
   pl->parts = static_cast<int>(cdiv64(nk, pl->split_width));
@@ -248,8 +249,7 @@ extern "C" int elsa_differential_backward(const void* q, const void* k, const vo
   if (rc != ELSA_OK) return rc;
   if (!q || !lam || !out || !out2 || !lse || !dout || !dq || !strides || (nk > 0 && (!k || !v || !dk || !dv)) || !dtype_ok(lam_dtype) || !scale_ok(scale))
     return ELSA_ERR_INVALID_ARGUMENT;
-  if (batch > 32767) return ELSA_ERR_UNSUPPORTED;
-  if (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 255u) || 
+  if (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 255u) ||
       workspace_bytes < diff_stats_bytes(batch, heads, nq) + diff_dlam_bytes(batch, heads, nq))
     return ELSA_ERR_WORKSPACE;
   auto st = static_cast<cudaStream_t>(stream);
@@ -261,7 +261,8 @@ extern "C" int elsa_differential_backward(const void* q, const void* k, const vo
   d.dlam = dlam;
   d.dlam_parts = dlam ? reinterpret_cast<float*>(static_cast<char*>(workspace) + diff_stats_bytes(batch, heads, nq)) : nullptr;
   float* stats = static_cast<float*>(workspace);
-  const bool tiles = diff_tc_sizes(dtype, head_dim, v_dim) && diff_inputs_in_tiles(d) && diff_rows_ok(dout, d.gs, v_dim, heads, batch) &&
+  // (the tile kernel has two bodies for each sequence in a grid of 65535)
+  const bool tiles = batch <= 32767 && diff_tc_sizes(dtype, head_dim, v_dim) && diff_inputs_in_tiles(d) && diff_rows_ok(dout, d.gs, v_dim, heads, batch) &&
                      diff_rows_ok(dq, d.dqs, head_dim, 2 * heads, batch) &&
                      (nk == 0 || (diff_rows_ok(dk, d.dks, head_dim, 2 * kv_heads, batch) && diff_rows_ok(dv, d.dvs, v_dim, kv_heads, batch)));
   if (tiles && (rc = device_status_ok()) != ELSA_OK) return rc;

@@ -252,7 +252,7 @@ bool diff_covers(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, 
   for (const at::Tensor* t : {&q, &k, &v})
     if (!plain(*t) || t->dim() != 4 || t->numel() == 0 || t->scalar_type() != q.scalar_type() || t->device() != q.device() || !row_strides(*t, st)) return false;
   c->dt = dtype_code(q.scalar_type());
-  if (c->dt < 0 || q.size(1) % 2 || k.size(1) % 2 || q.size(1) > 65535 || q.size(0) > 32767) return false;
+  if (c->dt < 0 || q.size(1) % 2 || k.size(1) % 2 || q.size(1) > 65535 || q.size(0) > 65535) return false;
   c->batch = static_cast<int>(q.size(0)); c->heads = static_cast<int>(q.size(1) / 2); c->kv_heads = static_cast<int>(k.size(1) / 2);
   c->nq = static_cast<int>(q.size(2)); c->nk = static_cast<int>(k.size(2)); c->d = static_cast<int>(q.size(3)); c->dv = static_cast<int>(v.size(3));
   if (k.size(0) != c->batch || v.size(0) != c->batch || k.size(3) != c->d || v.size(1) != c->kv_heads || v.size(2) != c->nk ||

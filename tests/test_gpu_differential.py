@@ -438,3 +438,12 @@ def test_a_scale_that_fp32_does_not_hold_is_refused(scale):
     for call in (E.differential_attention, E.differential_attention_train):
         with pytest.raises(ValueError, match="scale"):
             call(q, k, v, lam, is_causal=True, scale=scale)
+
+
+def test_training_with_more_sequences_than_the_tile_kernels_grid():
+    q, k, v, lam = _inputs(33000, 1, 1, 1, 2, 8, 8, torch.float16)
+    dout = _normal((33000, 1, 1, 8), torch.float16, 9)
+    out, got = _run_train(q, k, v, lam, dout)
+    for rows in (slice(0, 20), slice(32980, 33000)):
+        _check_forward(out[rows], q[rows], k[rows], v[rows], lam)
+        _check_gradients([g[rows] for g in got[:3]], q[rows], k[rows], v[rows], lam, dout[rows])
