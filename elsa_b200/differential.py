@@ -12,7 +12,7 @@ import torch
 
 from . import _lib
 from .attention import _DeviceScope, _aligned, _cached_bytes, _in_place_or_copy
-from .rotary import _MAX_SIZE, _check_saved, _check_sizes, _once_differentiable
+from .rotary import _MAX_SIZE, _check_saved, _check_sizes, _once_differentiable, _refuse_transforms
 from .shared_prefix import _check_lengths, _positive_scale, _readable, _strides
 
 
@@ -122,6 +122,7 @@ def differential_attention(
     sizes = _check(q, k, v, lam, "differential_attention")
     _check_lengths(lengths, sizes[0], q.device)
     scale = _positive_scale(scale, sizes[5])
+    _refuse_transforms("differential_attention", q, k, v, *((lam,) if isinstance(lam, torch.Tensor) else ()))
     if sizes[0] * sizes[1] * sizes[3] * sizes[6] == 0:
         return torch.empty((sizes[0], sizes[1], sizes[3], sizes[6]), device=q.device, dtype=q.dtype)
     return _forward(q, k, v, lam, sizes, is_causal, scale, lengths, False)[0]

@@ -83,6 +83,15 @@ def rotary_frequencies(
     return frequencies.to(device) if device is not None else frequencies, magnitude
 
 
+def _refuse_transforms(who: str, *tensors):
+    """An operator without an autograd function of its own is neither recorded by torch.jit.trace (the trace would hold its memory, not
+    its work) nor given a tangent by forward-mode differentiation: it says so."""
+    if torch.jit.is_tracing():
+        raise RuntimeError(f"{who} cannot be recorded by torch.jit.trace")
+    if any(torch.autograd.forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        raise NotImplementedError(f"{who} has no forward-mode derivative")
+
+
 def _row_strides(t: torch.Tensor):
     """(batch, head, row) element strides, or None where the D axis is not contiguous."""
     b, h, n, d = t.shape
@@ -278,6 +287,7 @@ def rotary_embedding(
         frequencies = frequencies.contiguous()
     magnitude = float(magnitude)
     if inplace:
+        _refuse_transforms("rotary_embedding(inplace=True)", q, *(() if k is None else (k,)))
         if torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad)):
             raise ValueError("inplace=True has no gradients: use it under torch.no_grad()")
         for t in (q,) if k is None else (q, k):

@@ -13,7 +13,7 @@ import torch
 
 from . import _lib
 from .attention import _DeviceScope, _cached_bytes, _empty_like_layout
-from .rotary import _check_sizes
+from .rotary import _check_sizes, _refuse_transforms
 
 
 def _strides(t: torch.Tensor):
@@ -96,6 +96,7 @@ def shared_prefix_attention(
         raise ValueError("head_dim > 128 is not supported by the current kernels")
     _check_lengths(lengths, batch, q.device)
     scale = _positive_scale(scale, dim)
+    _refuse_transforms("shared_prefix_attention", q, k_prefix, v_prefix, k, v)
     if q.numel() == 0:
         return torch.empty_like(q)
     n_prefix, n_own = int(k_prefix.shape[1]), int(k.shape[2])

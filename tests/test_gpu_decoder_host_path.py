@@ -142,6 +142,24 @@ def test_a_traced_call_follows_its_inputs(entry, grad):
         _assert_equal(traced(*other), call(*other))
 
 
+@pytest.mark.parametrize("op", ["shared_prefix", "differential", "rotary_inplace"])
+def test_forward_only_operators_refuse_traces_and_tangents(op, path):
+    """A trace would hold their memory and not their work, a dual number's result no tangent."""
+    inputs = {"shared_prefix": [_normal((3, 4, 2, 64), 1), _normal((2, 50, 64), 2), _normal((2, 50, 64), 3), _normal((3, 2, 30, 64), 4), _normal((3, 2, 30, 64), 5)],
+              "differential": [_normal((3, 4, 2, 64), 4), _normal((3, 2, 40, 64), 5), _normal((3, 1, 40, 96), 6), torch.tensor([0.3, 0.6], device="cuda")],
+              "rotary_inplace": [_normal((2, 4, 70, 64), 1), _normal((2, 2, 70, 64), 2)]}[op]
+    f = E.rotary_frequencies(32, device="cuda")[0]
+    call = {"shared_prefix": E.shared_prefix_attention, "differential": E.differential_attention,
+            "rotary_inplace": lambda q, k: E.rotary_embedding(q, k, f, inplace=True)}[op]
+    with pytest.raises(RuntimeError, match="torch.jit.trace"):
+        torch.jit.trace(call, tuple(inputs), check_trace=False)
+    for i in range(len(inputs)):
+        with torch.autograd.forward_ad.dual_level():
+            dual = [torch.autograd.forward_ad.make_dual(t, torch.ones_like(t)) if j == i else t for j, t in enumerate(inputs)]
+            with pytest.raises(NotImplementedError):
+                call(*dual)
+
+
 @pytest.mark.parametrize("entry", ENTRIES)
 def test_a_second_derivative_is_refused_not_dropped(entry, path):
     inputs, call, grads = _problem(entry)
