@@ -62,12 +62,23 @@ int plan_prefix(int dtype, int batch, int heads, int kv_heads, int nq, int head_
     pl->own_parts = static_cast<int>(cdiv64(n_own, pl->own_width));
   }
   if (pl->tiles) {
-    // one CTA for each 256 rows, key head and part, one CTA on an SM: waves x (64-key tiles of a part + what a CTA costs besides, about
-    // eight of them)
-    const int64_t ctas = cdiv64(rows, 256) * kv_heads, tiles = cdiv64(n_prefix, 64);
-    int64_t best = 0, best_cost = 0;
+    // One CTA for each 256 rows, key head and part, one CTA on an SM: waves x (64-key tiles of a part + what a CTA costs besides, about
+    // 18 of them).  The split kernel of the sequences' own keys runs beside it, on the SMs that it leaves free: about 0.7 of them read at
+    // full speed, fewer in proportion.  So few parts may be the best, a prefix that takes long on some SMs while the caches stream
+    // through the others.  Measured (head dim 128, bf16): 256 sequences with 2048 keys behind 32768, 32 CTAs a part: 252 us with 2 parts,
+    // 271 with 3, 306 with 9 (two full waves, then the caches; under the power cap of a long run 307, 312, 336); 64 with 1024 behind 8192, 8 CTAs a part: 56 us with 7 parts, 69
+    // with 4, 67 with 18; 24 x 3 with 333 behind 4097, 6 CTAs a part: 29.7 us with 13, 33.8 with 17, 35.9 with 22.  (With caches all but
+    // empty the first of these loses, 241 us against 198 one after the other; half full it is 247 against 280, full 335 against 386.)
+    const double tile_us = 0.8, bytes_us = 6.3e6;
+    const double own = n_own > 0 ? (2.0 * head_dim * batch * kv_heads * n_own / bytes_us + 9.0) / tile_us : 0.0;    // in tiles too, of caches half full
+    const int64_t ctas = cdiv64(rows, 256) * kv_heads, tiles = cdiv64(n_prefix, 64), sms = sm_count();
+    int64_t best = 0;
+    double best_cost = 0.0;
     for (int64_t parts = 1; parts <= std::min<int64_t>(tiles, 64); ++parts) {
-      const int64_t per = cdiv64(tiles, parts), cost = cdiv64(ctas * cdiv64(tiles, per), sm_count()) * (per + 8);
+      const int64_t per = cdiv64(tiles, parts), all = ctas * cdiv64(tiles, per);
+      const double prefix = static_cast<double>(cdiv64(all, sms) * (per + 18));
+      const double beside = prefix * std::min(1.0, std::max<int64_t>(0, sms - all) / (0.7 * sms));    // of the caches, while the prefix takes its time
+      const double cost = prefix + std::max(0.0, own - beside);
       if (best == 0 || cost < best_cost) { best = per; best_cost = cost; }
     }
     pl->prefix_width = static_cast<int>(best * 64);
@@ -170,6 +181,7 @@ extern "C" int elsa_shared_prefix_attention(const void* q, const void* k_prefix,
   p.z = reinterpret_cast<float*>(ws + pl.mz_bytes);
   p.s = reinterpret_cast<float*>(ws + 2 * pl.mz_bytes);
   p.out = out; p.os = Strides{strides[13], strides[14], strides[15]};
+  bool beside = false;                                  // the prefix's kernel has been launched
   if (n_prefix > 0) {
     DecodeSegment& s = p.seg[0];
     s.k = k_prefix; s.v = v_prefix; s.ks = Strides{0, strides[3], strides[4]}; s.vs = Strides{0, strides[5], strides[6]}; s.n_keys = n_prefix; s.shared = 1;
@@ -178,6 +190,7 @@ extern "C" int elsa_shared_prefix_attention(const void* q, const void* k_prefix,
     if (pl.tiles && rows_tc_ok(p, dtype)) {
       if ((rc = device_status_ok()) != ELSA_OK) return rc;
       if ((rc = rows_tc(p, pl.prefix_width, pl.prefix_parts, dtype, st)) != ELSA_OK) return rc;
+      beside = true;
     } else {
       p.n_segs = 1;
     }
@@ -189,8 +202,8 @@ extern "C" int elsa_shared_prefix_attention(const void* q, const void* k_prefix,
     s.lengths = lengths; s.n_keys = n_own; s.causal = 1;
     s.split_width = pl.own_width; s.n_splits = pl.own_parts; s.first_part = pl.prefix_parts;
   }
-  if ((rc = decode_split(p, dtype, st)) != ELSA_OK) return rc;
-  return decode_merge(p, pl.prefix_parts + pl.own_parts, dtype, st);
+  if ((rc = decode_split(p, dtype, beside, st)) != ELSA_OK) return rc;
+  return decode_merge(p, pl.prefix_parts + pl.own_parts, dtype, n_prefix + n_own > 0, st);
 }
 
 extern "C" int64_t elsa_differential_workspace_bytes(int dtype, int batch, int heads, int kv_heads, int nq, int nk, int head_dim, int v_dim) {
@@ -229,8 +242,8 @@ extern "C" int elsa_differential_forward(const void* q, const void* k, const voi
     s.k = k; s.v = v; s.ks = d.ks; s.vs = d.vs; s.lengths = lengths; s.n_keys = nk; s.causal = is_causal;
     s.split_width = pl.split_width; s.n_splits = pl.parts;
   }
-  if ((rc = decode_split(p, dtype, st)) != ELSA_OK) return rc;
-  return decode_merge(p, pl.parts, dtype, st);
+  if ((rc = decode_split(p, dtype, false, st)) != ELSA_OK) return rc;
+  return decode_merge(p, pl.parts, dtype, nk > 0, st);
 }
 
 extern "C" int64_t elsa_differential_backward_workspace_bytes(int dtype, int batch, int heads, int kv_heads, int nq, int nk, int head_dim,

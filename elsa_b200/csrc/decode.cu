@@ -9,8 +9,14 @@
 //                      with running max, sum and O in registers; the four are merged through shared memory at the end.  mma.sync
 //                      and not tcgen05: a tile has 16 rows here and not 128, a warp's products stay in its registers, and 8
 //                      bytes are loaded for every row's multiply-add that either could do.
+//                      A warp needs about 2300 cycles for 16 keys, a chain of products, shuffles and exponentials: with eight warps an
+//                      SM reads 52 GB/s, and about 0.7 of the SMs are enough for the memory's rate.
 //   split_any_kernel   any type, any head dim up to 128, any stride, in fp32 (split tf32 operands) on 32 x 32 tiles.
-//   merge_kernel       a warp per row.
+//   merge_kernel       a warp per row, on the device early (it waits for the launch before it): 1 us less for a call.
+//
+// Measured, bf16, head dim 128: 256 x 8 caches of up to 2048 keys, 1.1 GB, 172 us = 6.3 TB/s, 0.96 of a plain copy's rate; 16 x 4
+// caches of up to 8192 keys of two maps (head dim 64, values of 128), 167 MB, 43 us: about 310 blocks of 960 keys in 296 places, 1.05
+// waves that take the time of two (33 to 46 us with 256 to 2048 keys a block, by chance).
 //
 // Softmax statistics, sums and O are fp32; P is rounded to the inputs' type for the second product (its error, half a step of
 // that type in each weight, averages out over the keys).  The reference max of a row moves only when it is exceeded by more than
@@ -63,6 +69,11 @@ __device__ __forceinline__ int64_t q_offset(const DecodeParams& p, int g, int ro
   return b * p.qs.b + static_cast<int64_t>(p.maps * (g * group + gi) + map) * p.qs.h + i * p.qs.r;
 }
 
+// The last block ends after the launch before this one: what waits for this launch has waited for that one too.
+__device__ __forceinline__ void end_behind_previous() {
+  if (blockIdx.x == gridDim.x - 1 && threadIdx.x == 0) wait_for_previous();
+}
+
 // ---- tensor cores -----------------------------------------------------------------------------------------------------
 template <typename T>
 __device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1);
@@ -102,7 +113,11 @@ split_mma_kernel(const DecodeParams p) {
   using Tile = MmaTile<MAPS, DP, VP>;
   extern __shared__ __align__(16) uint8_t smem[];
   Block w;
-  if (!locate(p, kMmaRows, w)) return;
+  let_next_begin();
+  if (!locate(p, kMmaRows, w)) {
+    end_behind_previous();
+    return;
+  }
   const DecodeSegment& sg = p.seg[w.seg];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, quad = lane & 3, qrow = lane >> 2;
   const uint32_t ring = tc::smem_u32(smem) + warp * kStages * Tile::kStage;
@@ -120,26 +135,48 @@ split_mma_kernel(const DecodeParams p) {
   }
   const int n_chunks = (w.k1 - w.k0 + kMmaKeys - 1) / kMmaKeys;
   const int mine = n_chunks > warp ? (n_chunks - warp + kMmaWarps - 1) / kMmaWarps : 0;   // chunks warp, warp + 4, ...
+  // A lane copies one 16-byte piece of every kPassK-th (kPassV-th) key of a chunk.  Chunks come in order: the sources move on by as much each
+  // time.  Keys beyond the last one (of the last chunk): nothing is read, zeros are written.
+  constexpr int kPassK = 256 / DP, kPassV = 256 / VP;    // keys of one pass of the warp
+  const int k_row = lane / (DP / 8), k_col = lane % (DP / 8), v_row = lane / (VP / 8), v_col = lane % (VP / 8);
+  const bool k_real = k_col < d_pieces, v_real = v_col < v_pieces;
+  const int64_t k_pass = kPassK * sg.ks.r, v_pass = kPassV * sg.vs.r, k_step = kMmaWarps * kMmaKeys * sg.ks.r, v_step = kMmaWarps * kMmaKeys * sg.vs.r;
+  int next = w.k0 + warp * kMmaKeys;                     // first key of the next chunk
+#pragma unroll
+  for (int m = 0; m < MAPS; ++m) kp[m] += (next + k_row) * sg.ks.r + k_col * 8;
+  vp += (next + v_row) * sg.vs.r + v_col * 8;
+  const uint32_t k_dst = k_row * Tile::kPitchK + k_col * 16, v_dst = MAPS * kMmaKeys * Tile::kPitchK + v_row * Tile::kPitchV + v_col * 16;
   auto copy = [&](int it) {
     if (it < mine) {
       const uint32_t st = ring + (it % kStages) * Tile::kStage;
-      const int key0 = w.k0 + (warp + it * kMmaWarps) * kMmaKeys;
+      const int valid = w.k1 - next;
+      if (valid >= kMmaKeys) {
 #pragma unroll
-      for (int m = 0; m < MAPS; ++m) {
+        for (int m = 0; m < MAPS; ++m)
 #pragma unroll
-        for (int i = 0; i < kMmaKeys * DP / 8; i += 32) {
-          const int r = (i + lane) / (DP / 8), c = (i + lane) % (DP / 8), key = key0 + r;
-          // (keys beyond the last one: nothing is read, zeros are written)
-          if (c < d_pieces)
-            cp16(st + m * kMmaKeys * Tile::kPitchK + r * Tile::kPitchK + c * 16, kp[m] + static_cast<int64_t>(min(key, w.k1 - 1)) * sg.ks.r + c * 8, key < w.k1 ? 16 : 0);
+          for (int i = 0; i < kMmaKeys / kPassK; ++i)
+            if (k_real) cp16(st + k_dst + (m * kMmaKeys + i * kPassK) * Tile::kPitchK, kp[m] + i * k_pass, 16);
+#pragma unroll
+        for (int i = 0; i < kMmaKeys / kPassV; ++i)
+          if (v_real) cp16(st + v_dst + i * kPassV * Tile::kPitchV, vp + i * v_pass, 16);
+      } else {
+#pragma unroll
+        for (int m = 0; m < MAPS; ++m)
+#pragma unroll
+          for (int i = 0; i < kMmaKeys / kPassK; ++i) {
+            const bool there = i * kPassK + k_row < valid;
+            if (k_real) cp16(st + k_dst + (m * kMmaKeys + i * kPassK) * Tile::kPitchK, there ? kp[m] + i * k_pass : static_cast<const T*>(sg.k), there ? 16 : 0);
+          }
+#pragma unroll
+        for (int i = 0; i < kMmaKeys / kPassV; ++i) {
+          const bool there = i * kPassV + v_row < valid;
+          if (v_real) cp16(st + v_dst + i * kPassV * Tile::kPitchV, there ? vp + i * v_pass : static_cast<const T*>(sg.v), there ? 16 : 0);
         }
       }
 #pragma unroll
-      for (int i = 0; i < kMmaKeys * VP / 8; i += 32) {
-        const int r = (i + lane) / (VP / 8), c = (i + lane) % (VP / 8), key = key0 + r;
-        if (c < v_pieces)
-          cp16(st + MAPS * kMmaKeys * Tile::kPitchK + r * Tile::kPitchV + c * 16, vp + static_cast<int64_t>(min(key, w.k1 - 1)) * sg.vs.r + c * 8, key < w.k1 ? 16 : 0);
-      }
+      for (int m = 0; m < MAPS; ++m) kp[m] += k_step;
+      vp += v_step;
+      next += kMmaWarps * kMmaKeys;
     }
     asm volatile("cp.async.commit_group;" ::: "memory");   // (an empty group keeps the count)
   };
@@ -153,7 +190,7 @@ split_mma_kernel(const DecodeParams p) {
   for (int half = 0; half < 2; ++half) {
     const int r = qrow + 8 * half;
     const bool real = r < w.n_rows;
-    lim[half] = real ? row_limit(p, sg, w.len, w.row0 + r) : 0;
+    lim[half] = real ? min(w.k1, row_limit(p, sg, w.len, w.row0 + r)) : w.k1;
 #pragma unroll
     for (int m = 0; m < MAPS; ++m) {
       const T* qp = static_cast<const T*>(p.q) + (real ? q_offset(p, w.g, w.row0 + r, m) : 0);
@@ -179,13 +216,14 @@ split_mma_kernel(const DecodeParams p) {
   const uint32_t k_lane = ((lane & 7) + ((lane >> 4) << 3)) * Tile::kPitchK + ((lane >> 3) & 1) * 16;
   const uint32_t v_lane = ((lane & 7) + (((lane >> 3) & 1) << 3)) * Tile::kPitchV + (lane >> 4) * 16;
   const float c = p.scale_log2;
+  const int seen = __reduce_min_sync(0xffffffffu, min(lim[0], lim[1]));      // keys before it are seen by every row
 
   for (int it = 0; it < mine; ++it) {
     asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 2) : "memory");
     __syncwarp();                                       // every lane's copies of this stage are there, and the stage before it has been read
     copy(it + kStages - 1);                             // over that one: two stages are on their way while this one is used
     const uint32_t st = ring + (it % kStages) * Tile::kStage;
-    const int key0 = w.k0 + (warp + it * kMmaWarps) * kMmaKeys + quad * 2;
+    const int chunk0 = w.k0 + (warp + it * kMmaWarps) * kMmaKeys;
     uint32_t pf[MAPS][4];
 #pragma unroll
     for (int m = 0; m < MAPS; ++m) {
@@ -197,18 +235,18 @@ split_mma_kernel(const DecodeParams p) {
         mma16816<T>(s[0], qf[m][kk], kf[0], kf[1]);
         mma16816<T>(s[1], qf[m][kk], kf[2], kf[3]);
       }
-      float top[2] = {-CUDART_INF_F, -CUDART_INF_F};
+      if (chunk0 + kMmaKeys > seen) {
 #pragma unroll
-      for (int n = 0; n < 2; ++n)
+        for (int n = 0; n < 2; ++n)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const int key = key0 + n * 8 + (e & 1);
-          s[n][e] = key < min(lim[e >> 1], w.k1) ? s[n][e] * c : -CUDART_INF_F;
-          top[e >> 1] = fmaxf(top[e >> 1], s[n][e]);
-        }
+          for (int e = 0; e < 4; ++e)
+            if (chunk0 + quad * 2 + n * 8 + (e & 1) >= lim[e >> 1]) s[n][e] = -CUDART_INF_F;
+      }
+      float top[2];
       bool move[2];
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
+        top[h] = fmaxf(fmaxf(s[0][2 * h], s[0][2 * h + 1]), fmaxf(s[1][2 * h], s[1][2 * h + 1])) * c;
         top[h] = fmaxf(top[h], __shfl_xor_sync(0xffffffffu, top[h], 1));
         top[h] = fmaxf(top[h], __shfl_xor_sync(0xffffffffu, top[h], 2));
         move[h] = top[h] > m_ref[m][h] + kRescaleThreshold;
@@ -229,9 +267,9 @@ split_mma_kernel(const DecodeParams p) {
       }
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        const float m_use = m_ref[m][h] == -CUDART_INF_F ? 0.f : m_ref[m][h];
-        float e0 = fast_exp2(s[0][2 * h] - m_use), e1 = fast_exp2(s[0][2 * h + 1] - m_use);
-        float e2 = fast_exp2(s[1][2 * h] - m_use), e3 = fast_exp2(s[1][2 * h + 1] - m_use);
+        const float nm = m_ref[m][h] == -CUDART_INF_F ? 0.f : -m_ref[m][h];
+        const float e0 = fast_exp2(fmaf(s[0][2 * h], c, nm)), e1 = fast_exp2(fmaf(s[0][2 * h + 1], c, nm));
+        const float e2 = fast_exp2(fmaf(s[1][2 * h], c, nm)), e3 = fast_exp2(fmaf(s[1][2 * h + 1], c, nm));
         z[m][h] += (e0 + e1) + (e2 + e3);
         pf[m][h] = tc::pack2<T>(e0, e1);
         pf[m][2 + h] = tc::pack2<T>(e2, e3);
@@ -289,6 +327,7 @@ split_mma_kernel(const DecodeParams p) {
       p.z[at] = zs;
     }
   }
+  end_behind_previous();
 }
 
 // ---- any type ---------------------------------------------------------------------------------------------------------
@@ -304,7 +343,11 @@ split_any_kernel(const DecodeParams p) {
   float* sk = sq + MAPS * kAnyRows * kPitch;            // [map][key][dim]
   float* sv = sk + MAPS * kAnyKeys * kPitch;            // [key][dim]
   Block w;
-  if (!locate(p, kAnyRows, w)) return;
+  let_next_begin();
+  if (!locate(p, kAnyRows, w)) {
+    end_behind_previous();
+    return;
+  }
   const DecodeSegment& sg = p.seg[w.seg];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, half = warp & 1, map = MAPS == 2 ? warp >> 1 : 0, part = MAPS == 2 ? 0 : warp >> 1;
   const int d8 = (p.head_dim + 7) / 8 * 8, v8 = (p.v_dim + 7) / 8 * 8;
@@ -439,6 +482,7 @@ split_any_kernel(const DecodeParams p) {
       p.z[at] = z[j];
     }
   }
+  end_behind_previous();
 }
 
 // ---- merge ------------------------------------------------------------------------------------------------------------
@@ -453,6 +497,7 @@ merge_kernel(const DecodeParams p, int n_parts) {
   const int i = blockIdx.x * 4 + (threadIdx.x >> 5);
   const int lane = threadIdx.x & 31;
   if (i >= rows * p.kv_heads) return;
+  wait_for_previous();
   const int g = i / static_cast<int>(rows), row = i - g * static_cast<int>(rows);
   const int group = p.heads / p.kv_heads, per = group * p.nq;
   const int b = row / per, r = row - b * per, gi = r / p.nq, t = r - gi * p.nq, h = g * group + gi;
@@ -475,11 +520,11 @@ merge_kernel(const DecodeParams p, int n_parts) {
     for (int u = 0; u < kAhead; ++u) {
       const float* src = ps + min(p0 + u, n_parts - 1) * step * p.v_dim;
       if (VEC == 4) {
-        const float4 v = lane * 4 < p.v_dim ? *reinterpret_cast<const float4*>(src) : make_float4(0.f, 0.f, 0.f, 0.f);
+        const float4 v = lane * 4 < p.v_dim ? __ldcg(reinterpret_cast<const float4*>(src)) : make_float4(0.f, 0.f, 0.f, 0.f);
         x[u][0] = v.x; x[u][1] = v.y; x[u][2] = v.z; x[u][3] = v.w;
       } else {
 #pragma unroll
-        for (int e = 0; e < kCols; ++e) x[u][e] = lane + 32 * e < p.v_dim ? src[32 * e] : 0.f;
+        for (int e = 0; e < kCols; ++e) x[u][e] = lane + 32 * e < p.v_dim ? __ldcg(src + 32 * e) : 0.f;
       }
     }
   };
@@ -495,8 +540,8 @@ merge_kernel(const DecodeParams p, int n_parts) {
       load8(x, ps, p0);                                 // (beside the weights: one latency less)
       float m_part = -CUDART_INF_F, z_part = 0.f;
       if (p0 + lane < n_parts && written(p0 + lane)) {
-        m_part = pm[(p0 + lane) * step];
-        z_part = pz[(p0 + lane) * step];
+        m_part = __ldcg(pm + (p0 + lane) * step);
+        z_part = __ldcg(pz + (p0 + lane) * step);
       }
       float best = m_part;
 #pragma unroll
@@ -557,30 +602,26 @@ merge_kernel(const DecodeParams p, int n_parts) {
 }
 
 template <typename T, int MAPS, int DP, int VP>
-int launch_mma(const DecodeParams& p, int64_t blocks, cudaStream_t st) {
+int launch_mma(const DecodeParams& p, int64_t blocks, bool behind, cudaStream_t st) {
   const auto kernel = &split_mma_kernel<T, MAPS, DP, VP>;
   const int rc = ensure_dynamic_smem(reinterpret_cast<const void*>(kernel), MmaTile<MAPS, DP, VP>::kSmem);
   if (rc != ELSA_OK) return rc;
-  kernel<<<static_cast<unsigned>(blocks), kMmaThreads, MmaTile<MAPS, DP, VP>::kSmem, st>>>(p);
-  ELSA_LAUNCH_CHECK();
-  return ELSA_OK;
+  return launch_behind(behind, kernel, static_cast<unsigned>(blocks), kMmaThreads, MmaTile<MAPS, DP, VP>::kSmem, st, p);
 }
 
 template <typename T>
-int launch_mma_t(const DecodeParams& p, int64_t blocks, cudaStream_t st) {
-  if (p.maps == 2) return p.v_dim > 64 ? launch_mma<T, 2, 64, 128>(p, blocks, st) : launch_mma<T, 2, 64, 64>(p, blocks, st);
-  return p.head_dim > 64 || p.v_dim > 64 ? launch_mma<T, 1, 128, 128>(p, blocks, st) : launch_mma<T, 1, 64, 64>(p, blocks, st);
+int launch_mma_t(const DecodeParams& p, int64_t blocks, bool behind, cudaStream_t st) {
+  if (p.maps == 2) return p.v_dim > 64 ? launch_mma<T, 2, 64, 128>(p, blocks, behind, st) : launch_mma<T, 2, 64, 64>(p, blocks, behind, st);
+  return p.head_dim > 64 || p.v_dim > 64 ? launch_mma<T, 1, 128, 128>(p, blocks, behind, st) : launch_mma<T, 1, 64, 64>(p, blocks, behind, st);
 }
 
 template <typename T>
-int launch_any_t(const DecodeParams& p, int64_t blocks, cudaStream_t st) {
+int launch_any_t(const DecodeParams& p, int64_t blocks, bool behind, cudaStream_t st) {
   const auto kernel = p.maps == 2 ? &split_any_kernel<T, 2> : &split_any_kernel<T, 1>;
   const int smem = 4 * (p.maps * (kAnyRows + kAnyKeys) + kAnyKeys) * (kAnyDim + 4);
   const int rc = ensure_dynamic_smem(reinterpret_cast<const void*>(kernel), smem);
   if (rc != ELSA_OK) return rc;
-  kernel<<<static_cast<unsigned>(blocks), kAnyThreads, smem, st>>>(p);
-  ELSA_LAUNCH_CHECK();
-  return ELSA_OK;
+  return launch_behind(behind, kernel, static_cast<unsigned>(blocks), kAnyThreads, smem, st, p);
 }
 
 }  // namespace
@@ -598,7 +639,7 @@ bool decode_mma_ok(const DecodeParams& p, int dtype) {
   return true;
 }
 
-int decode_split(DecodeParams& p, int dtype, cudaStream_t st) {
+int decode_split(DecodeParams& p, int dtype, bool behind, cudaStream_t st) {
   if (p.head_dim > kAnyDim || p.v_dim > kAnyDim) return ELSA_ERR_UNSUPPORTED;
   const bool mma = decode_mma_ok(p, dtype);
   const int tile = mma ? kMmaRows : kAnyRows;
@@ -612,25 +653,23 @@ int decode_split(DecodeParams& p, int dtype, cudaStream_t st) {
   }
   if (blocks == 0) return ELSA_OK;
   if (blocks > 0x7fffffffll) return ELSA_ERR_UNSUPPORTED;
-  if (mma) return dtype == ELSA_F16 ? launch_mma_t<__half>(p, blocks, st) : launch_mma_t<__nv_bfloat16>(p, blocks, st);
-  if (dtype == ELSA_F32) return launch_any_t<float>(p, blocks, st);
-  return dtype == ELSA_F16 ? launch_any_t<__half>(p, blocks, st) : launch_any_t<__nv_bfloat16>(p, blocks, st);
+  if (mma) return dtype == ELSA_F16 ? launch_mma_t<__half>(p, blocks, behind, st) : launch_mma_t<__nv_bfloat16>(p, blocks, behind, st);
+  if (dtype == ELSA_F32) return launch_any_t<float>(p, blocks, behind, st);
+  return dtype == ELSA_F16 ? launch_any_t<__half>(p, blocks, behind, st) : launch_any_t<__nv_bfloat16>(p, blocks, behind, st);
 }
 
 template <typename T>
-static int merge_t(const DecodeParams& p, int n_parts, unsigned grid, cudaStream_t st) {
+static int merge_t(const DecodeParams& p, int n_parts, unsigned grid, bool behind, cudaStream_t st) {
   const bool vec = p.v_dim % 4 == 0;                    // (the sums start on a 256-byte boundary)
   const auto kernel = p.maps == 2 ? (vec ? &merge_kernel<T, 2, 4> : &merge_kernel<T, 2, 1>) : (vec ? &merge_kernel<T, 1, 4> : &merge_kernel<T, 1, 1>);
-  kernel<<<grid, 128, 0, st>>>(p, n_parts);
-  ELSA_LAUNCH_CHECK();
-  return ELSA_OK;
+  return launch_behind(behind, kernel, grid, 128, 0, st, p, n_parts);
 }
 
-int decode_merge(const DecodeParams& p, int n_parts, int dtype, cudaStream_t st) {
+int decode_merge(const DecodeParams& p, int n_parts, int dtype, bool behind, cudaStream_t st) {
   if (decode_rows(p) * p.kv_heads > 0x3fffffff) return ELSA_ERR_UNSUPPORTED;
   const unsigned grid = static_cast<unsigned>(cdiv64(decode_rows(p) * p.kv_heads, 4));
-  if (dtype == ELSA_F32) return merge_t<float>(p, n_parts, grid, st);
-  return dtype == ELSA_F16 ? merge_t<__half>(p, n_parts, grid, st) : merge_t<__nv_bfloat16>(p, n_parts, grid, st);
+  if (dtype == ELSA_F32) return merge_t<float>(p, n_parts, grid, behind, st);
+  return dtype == ELSA_F16 ? merge_t<__half>(p, n_parts, grid, behind, st) : merge_t<__nv_bfloat16>(p, n_parts, grid, behind, st);
 }
 
 }  // namespace elsa

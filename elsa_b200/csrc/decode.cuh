@@ -38,11 +38,32 @@ struct DecodeParams {
 
 __host__ __device__ inline int64_t decode_rows(const DecodeParams& p) { return static_cast<int64_t>(p.batch) * (p.heads / p.kv_heads) * p.nq; }
 
+// A kernel that was launched by launch_behind may begin while the launch before it in the stream still runs, once all of that one's blocks
+// have called let_next_begin (or ended); wait_for_previous returns when it has ended and its writes can be read.  Both do nothing in
+// other launches.
+__device__ __forceinline__ void let_next_begin() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+__device__ __forceinline__ void wait_for_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
+template <typename... Params, typename... Args>
+int launch_behind(bool behind, void (*kernel)(Params...), unsigned grid, unsigned threads, size_t smem, cudaStream_t st, const Args&... args) {
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(grid); cfg.blockDim = dim3(threads); cfg.dynamicSmemBytes = smem; cfg.stream = st;
+  cfg.attrs = &attr; cfg.numAttrs = behind ? 1 : 0;
+  ELSA_CUDA_CHECK(cudaLaunchKernelEx(&cfg, kernel, args...));
+  ELSA_LAUNCH_CHECK();
+  return ELSA_OK;
+}
+
 // whether the tensor-core kernel takes this: 16-bit types, rows on 16-byte boundaries, head and value dims it has
 bool decode_mma_ok(const DecodeParams& p, int dtype);
-// summaries of all segments in one launch; parts that begin beyond a sequence's keys are not written
-int decode_split(DecodeParams& p, int dtype, cudaStream_t st);
-// all parts of a row merged (of a segment that is not shared: those that begin before the sequence's last key)
-int decode_merge(const DecodeParams& p, int n_parts, int dtype, cudaStream_t st);
+// summaries of all segments in one launch; parts that begin beyond a sequence's keys are not written.  behind: it may run beside the launch
+// before it, one of these files' that does not write what it reads
+int decode_split(DecodeParams& p, int dtype, bool behind, cudaStream_t st);
+// all parts of a row merged (of a segment that is not shared: those that begin before the sequence's last key).  behind: it may come
+// onto the device early; the launch before it is one of these files'
+int decode_merge(const DecodeParams& p, int n_parts, int dtype, bool behind, cudaStream_t st);
 
 }  // namespace elsa

@@ -139,6 +139,7 @@ pair_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant__ 
   auto bar_pv = [&](int t) { return bar0 + 8 * (10 + 2 * kStages + t); };                  // P_t V of tile j has retired
   auto bar_o = [&](int t) { return bar0 + 8 * (12 + 2 * kStages + t); };                   // ... of the last tile
 
+  if (MODE != kDiff) let_next_begin();                  // (the split kernel of the sequences' own keys, on the SMs that are free)
   if (tid == 0) {
     abort_flag = 0;
     mbar_init(bar_q, MODE == kDiff ? 1 : 8);

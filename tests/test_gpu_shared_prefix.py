@@ -223,3 +223,26 @@ def test_a_scale_that_fp32_does_not_hold_is_refused(scale):
     """(one that is zero there would turn masked scores into NaN)"""
     with pytest.raises(ValueError, match="scale"):
         E.shared_prefix_attention(*_inputs(2, 4, 2, 2, 64, 90, 20, torch.float16), scale=scale)
+
+
+@pytest.mark.parametrize("shape", [(40, 8, 2, 1, 64, 700, 300), (3, 8, 2, 1, 64, 700, 300), (24, 12, 3, 5, 96, 1000, 333)], ids=str)
+def test_calls_in_a_row_and_side_by_side_do_not_meet(shape):
+    """The kernels of a call overlap one another; those of the next call, or of one on another stream, must find nothing of theirs."""
+    calls = [_inputs(*shape, torch.float16) for _ in range(4)]
+    for i, args in enumerate(calls):
+        args[0].mul_(1 + i)
+        args[4].add_(i)
+    want = [E.shared_prefix_attention(*args) for args in calls]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    for _ in range(10):
+        row = [E.shared_prefix_attention(*args) for args in calls]
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(row, want))
+        beside = []
+        for i, args in enumerate(calls):
+            with torch.cuda.stream(streams[i % 2]):
+                beside.append(E.shared_prefix_attention(*args) * 1)
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(beside, want))
+
