@@ -31,8 +31,10 @@ int device_status_ok() {
 // splits as give two waves of two blocks on an SM, whose second wave evens out caches of different lengths.  Measured, bf16, head
 // dim 128: 256 x 8 caches of up to 2048 keys 174 us at 1024 keys a split, 238 at 256, 550 at 64; 64 x 8 of up to 1024 keys 33 us at
 // 512 or 1024, 49 at 128; 24 x 3 of up to 333 keys 8.9 us at 512, 9.3 at 128, 13.3 at 64.
-int split_width(int64_t blocks_of_one_split, int n_keys) {
-  const int64_t wanted = std::max<int64_t>(1, 4ll * sm_count() / blocks_of_one_split);
+// fp32: a block's time is in its products, and keys that a causal mask hides are left out tile by tile: eight blocks for each SM
+// ((1, 4 heads, 1000 tokens, 64 / 128, causal): 80 us at 128 keys a split, 127 at 512).
+int split_width(int dtype, int64_t blocks_of_one_split, int n_keys) {
+  const int64_t wanted = std::max<int64_t>(1, (dtype == ELSA_F32 ? 8ll : 4ll) * sm_count() / blocks_of_one_split);
   const int64_t width = align_up(cdiv64(n_keys, wanted), 64);
   return static_cast<int>(std::max<int64_t>(64, std::min<int64_t>(width, 1024)));
 }
@@ -57,8 +59,9 @@ int plan_prefix(int dtype, int batch, int heads, int kv_heads, int nq, int head_
   pl->rows = rows;
   pl->tiles = rows > kTileRows && n_prefix >= 128 && (fold_tc_supported(dtype, head_dim, false) || fold_tcw_supported(dtype, head_dim, false));
   pl->prefix_width = pl->prefix_parts = pl->own_width = pl->own_parts = 0;
+  const int tile = dtype == ELSA_F32 ? 32 : 16;          // rows of a block of the split kernels
   if (n_own > 0) {
-    pl->own_width = split_width(static_cast<int64_t>(batch) * kv_heads * cdiv64(heads / kv_heads * nq, 16), n_own);
+    pl->own_width = split_width(dtype, static_cast<int64_t>(batch) * kv_heads * cdiv64(heads / kv_heads * nq, tile), n_own);
     pl->own_parts = static_cast<int>(cdiv64(n_own, pl->own_width));
   }
   if (pl->tiles) {
@@ -83,7 +86,7 @@ int plan_prefix(int dtype, int batch, int heads, int kv_heads, int nq, int head_
     }
     pl->prefix_width = static_cast<int>(best * 64);
   } else if (n_prefix > 0) {
-    pl->prefix_width = split_width(kv_heads * cdiv64(rows, 16), n_prefix);
+    pl->prefix_width = split_width(dtype, kv_heads * cdiv64(rows, tile), n_prefix);
   }
   if (n_prefix > 0) pl->prefix_parts = static_cast<int>(cdiv64(n_prefix, pl->prefix_width));
   const int64_t summaries = static_cast<int64_t>(pl->prefix_parts + pl->own_parts) * kv_heads * rows;
@@ -112,7 +115,7 @@ int plan_diff(int dtype, int batch, int heads, int kv_heads, int nq, int nk, int
   // (nq: the backward's four statistics of a head are indexed in 32 bits)
   if (rows * kv_heads > 0x1fffffff || heads > 65535 || batch > 65535 || nk > 0x3fffffff || nq > 0xfffffff) return ELSA_ERR_UNSUPPORTED;
   pl->tensor_tiles = rows_b > kSplitRows && diff_tc_sizes(dtype, head_dim, v_dim);
-  pl->split_width = nk > 0 ? split_width(static_cast<int64_t>(batch) * kv_heads * cdiv64(rows_b, 16), nk) : 1;
+  pl->split_width = nk > 0 ? split_width(dtype, static_cast<int64_t>(batch) * kv_heads * cdiv64(rows_b, dtype == ELSA_F32 ? 32 : 16), nk) : 1;
   pl->parts = static_cast<int>(cdiv64(nk, pl->split_width));
   const int64_t summaries = 2 * static_cast<int64_t>(pl->parts) * kv_heads * rows;
   pl->mz_bytes = align_up(summaries * 4, 256);

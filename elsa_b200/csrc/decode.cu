@@ -55,7 +55,11 @@ __device__ __forceinline__ bool locate(const DecodeParams& p, int tile_rows, Blo
   w.k0 = split * sg.split_width;
   w.k1 = min(w.len, w.k0 + sg.split_width);
   w.part = sg.first_part + split;
-  return w.k0 < w.len;
+  if (w.k0 >= w.len) return false;
+  // keys that no row of the tile sees are left out (a tile that spans a query head's end has the last token); with none left the summary says so
+  const int last = (w.row0 + w.n_rows - 1) % p.nq;
+  if (sg.causal && last >= w.n_rows - 1) w.k1 = min(w.k1, max(w.k0, w.len - p.nq + last + 1));
+  return true;
 }
 
 // the first key that row `row` (numbered within its kv head) does not see
@@ -334,11 +338,19 @@ split_mma_kernel(const DecodeParams p) {
 // 32 rows x 32 keys in fp32, products on split tf32 operands (tf32.cuh).  Four warps: 16 rows each, and of two maps one, or of one
 // map's keys the first or the second 16 (whose summaries are merged at the end).  A warp's weights go from its score accumulators
 // straight into the second product.
-template <typename T, int MAPS>
+// DP, VP: head dims rounded up to 64 or 128.
+template <int MAPS, int DP, int VP> struct AnyShape {
+  static constexpr int kPitch = DP + 4, kVPitch = VP + 4;
+  static constexpr int kSmem = 4 * (MAPS * (kAnyRows + kAnyKeys) * kPitch + kAnyKeys * kVPitch);
+};
+
+template <typename T, int MAPS, int DP, int VP>
 __global__ void __launch_bounds__(kAnyThreads)
 split_any_kernel(const DecodeParams p) {
   extern __shared__ __align__(16) float fsmem[];
-  constexpr int kPitch = kAnyDim + 4, kBlocks = MAPS == 2 ? 4 : 2;     // 8-key blocks of a warp's scores
+  constexpr int kPitch = AnyShape<MAPS, DP, VP>::kPitch, kVPitch = AnyShape<MAPS, DP, VP>::kVPitch;
+  constexpr int kBlocks = MAPS == 2 ? 4 : 2;            // 8-key blocks of a warp's scores
+  static_assert(MAPS == 2 || VP <= DP, "the merge of the two halves of the keys goes over the rows of Q");
   float* sq = fsmem;                                    // [map][row][dim]
   float* sk = sq + MAPS * kAnyRows * kPitch;            // [map][key][dim]
   float* sv = sk + MAPS * kAnyKeys * kPitch;            // [key][dim]
@@ -358,22 +370,23 @@ split_any_kernel(const DecodeParams p) {
     for (int r = threadIdx.x / 8; r < kAnyRows; r += kAnyThreads / 8) {
       const bool real = r < w.n_rows;
       const T* src = static_cast<const T*>(p.q) + (real ? q_offset(p, w.g, w.row0 + r, m) : 0);
-      for (int col = kc; col < kAnyDim; col += 8) sq[(m * kAnyRows + r) * kPitch + col] = real && col < p.head_dim ? to_f32<T>(src[col]) : 0.f;
+      for (int col = kc; col < DP; col += 8) sq[(m * kAnyRows + r) * kPitch + col] = real && col < p.head_dim ? to_f32<T>(src[col]) : 0.f;
     }
-  using KeyRows = tf32::Rows<T, kAnyThreads, kAnyKeys, kAnyDim>;
+  using KeyRows = tf32::Rows<T, kAnyThreads, kAnyKeys, DP>;
+  using ValueRows = tf32::Rows<T, kAnyThreads, kAnyKeys, VP>;
   const int64_t k_base = (sg.shared ? 0 : w.b * sg.ks.b) + static_cast<int64_t>(MAPS * w.g) * sg.ks.h;
   const KeyRows k1(sg.k, k_base, sg.ks.r, w.k1, p.head_dim), k2(sg.k, k_base + (MAPS - 1) * sg.ks.h, sg.ks.r, w.k1, p.head_dim);
-  const KeyRows vr(sg.v, (sg.shared ? 0 : w.b * sg.vs.b) + static_cast<int64_t>(w.g) * sg.vs.h, sg.vs.r, w.k1, p.v_dim);
+  const ValueRows vr(sg.v, (sg.shared ? 0 : w.b * sg.vs.b) + static_cast<int64_t>(w.g) * sg.vs.h, sg.vs.r, w.k1, p.v_dim);
   const int row = 16 * half + (lane >> 2);              // and row + 8
   int lim[2];
-  float m_run[2] = {-CUDART_INF_F, -CUDART_INF_F}, z[2] = {0.f, 0.f}, o[kAnyDim / 8][4] = {};
+  float m_run[2] = {-CUDART_INF_F, -CUDART_INF_F}, z[2] = {0.f, 0.f}, o[VP / 8][4] = {};
 #pragma unroll
   for (int j = 0; j < 2; ++j) lim[j] = row + 8 * j < w.n_rows ? min(w.k1, row_limit(p, sg, w.len, w.row0 + row + 8 * j)) : 0;
   for (int key0 = w.k0; key0 < w.k1; key0 += kAnyKeys) {
     __syncthreads();
     k1.load(sk, kPitch, key0);
     if (MAPS == 2) k2.load(sk + kAnyKeys * kPitch, kPitch, key0);
-    vr.load(sv, kPitch, key0);
+    vr.load(sv, kVPitch, key0);
     __syncthreads();
     float s[kBlocks][4] = {};
     const float* a = sq + (map * kAnyRows + 16 * half) * kPitch;
@@ -408,7 +421,7 @@ split_any_kernel(const DecodeParams p) {
     }
     if (__any_sync(0xffffffffu, alpha[0] != 1.f || alpha[1] != 1.f)) {
 #pragma unroll
-      for (int n = 0; n < kAnyDim / 8; ++n)
+      for (int n = 0; n < VP / 8; ++n)
 #pragma unroll
         for (int e = 0; e < 4; ++e) o[n][e] *= alpha[e >> 1];
     }
@@ -424,9 +437,9 @@ split_any_kernel(const DecodeParams p) {
       tf32::Split x[4], y[2];
       tf32::acc_as_a(x, s[k]);
 #pragma unroll
-      for (int n = 0; n < kAnyDim / 8; ++n) {
+      for (int n = 0; n < VP / 8; ++n) {
         if (8 * n >= v8) continue;
-        tf32::load_b(y, sv + (16 * part + 8 * k) * kPitch + 8 * n, kPitch, lane);
+        tf32::load_b(y, sv + (16 * part + 8 * k) * kVPitch + 8 * n, kVPitch, lane);
         tf32::mma3(o[n], x, y);
       }
     }
@@ -443,23 +456,23 @@ split_any_kernel(const DecodeParams p) {
     if (part == 1) {
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
-        float* dst = buffer + (row + 8 * j) * kPitch;
+        float* dst = buffer + (row + 8 * j) * kVPitch;
 #pragma unroll
-        for (int n = 0; n < kAnyDim / 8; ++n) { dst[8 * n + c] = o[n][2 * j]; dst[8 * n + c + 1] = o[n][2 * j + 1]; }
-        if ((lane & 3) == 0) { dst[kAnyDim] = m_run[j]; dst[kAnyDim + 1] = z[j]; }
+        for (int n = 0; n < VP / 8; ++n) { dst[8 * n + c] = o[n][2 * j]; dst[8 * n + c + 1] = o[n][2 * j + 1]; }
+        if ((lane & 3) == 0) { dst[VP] = m_run[j]; dst[VP + 1] = z[j]; }
       }
     }
     __syncthreads();
     if (part == 1) return;                              // (no barrier follows)
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
-      const float* src = buffer + (row + 8 * j) * kPitch;
-      const float m2 = src[kAnyDim], z2 = src[kAnyDim + 1], m_new = fmaxf(m_run[j], m2);
+      const float* src = buffer + (row + 8 * j) * kVPitch;
+      const float m2 = src[VP], z2 = src[VP + 1], m_new = fmaxf(m_run[j], m2);
       const float f1 = z[j] != 0.f ? exp2f(m_run[j] - m_new) : 0.f, f2 = z2 != 0.f ? exp2f(m2 - m_new) : 0.f;
       z[j] = z[j] * f1 + z2 * f2;
       m_run[j] = m_new;
 #pragma unroll
-      for (int n = 0; n < kAnyDim / 8; ++n) {
+      for (int n = 0; n < VP / 8; ++n) {
         o[n][2 * j] = o[n][2 * j] * f1 + src[8 * n + c] * f2;
         o[n][2 * j + 1] = o[n][2 * j + 1] * f1 + src[8 * n + c + 1] * f2;
       }
@@ -471,7 +484,7 @@ split_any_kernel(const DecodeParams p) {
     if (row + 8 * j >= w.n_rows) continue;
     const int64_t at = (base + row + 8 * j) * MAPS + map;
 #pragma unroll
-    for (int n = 0; n < kAnyDim / 8; ++n)
+    for (int n = 0; n < VP / 8; ++n)
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
         const int col = 8 * n + 2 * (lane & 3) + e;
@@ -615,13 +628,19 @@ int launch_mma_t(const DecodeParams& p, int64_t blocks, bool behind, cudaStream_
   return p.head_dim > 64 || p.v_dim > 64 ? launch_mma<T, 1, 128, 128>(p, blocks, behind, st) : launch_mma<T, 1, 64, 64>(p, blocks, behind, st);
 }
 
+template <typename T, int MAPS, int DP, int VP>
+int launch_any(const DecodeParams& p, int64_t blocks, bool behind, cudaStream_t st) {
+  const auto kernel = &split_any_kernel<T, MAPS, DP, VP>;
+  const int rc = ensure_dynamic_smem(reinterpret_cast<const void*>(kernel), AnyShape<MAPS, DP, VP>::kSmem);
+  if (rc != ELSA_OK) return rc;
+  return launch_behind(behind, kernel, static_cast<unsigned>(blocks), kAnyThreads, AnyShape<MAPS, DP, VP>::kSmem, st, p);
+}
+
 template <typename T>
 int launch_any_t(const DecodeParams& p, int64_t blocks, bool behind, cudaStream_t st) {
-  const auto kernel = p.maps == 2 ? &split_any_kernel<T, 2> : &split_any_kernel<T, 1>;
-  const int smem = 4 * (p.maps * (kAnyRows + kAnyKeys) + kAnyKeys) * (kAnyDim + 4);
-  const int rc = ensure_dynamic_smem(reinterpret_cast<const void*>(kernel), smem);
-  if (rc != ELSA_OK) return rc;
-  return launch_behind(behind, kernel, static_cast<unsigned>(blocks), kAnyThreads, smem, st, p);
+  if (p.maps == 1) return p.head_dim > 64 || p.v_dim > 64 ? launch_any<T, 1, 128, 128>(p, blocks, behind, st) : launch_any<T, 1, 64, 64>(p, blocks, behind, st);
+  if (p.head_dim > 64) return launch_any<T, 2, 128, 128>(p, blocks, behind, st);
+  return p.v_dim > 64 ? launch_any<T, 2, 64, 128>(p, blocks, behind, st) : launch_any<T, 2, 64, 64>(p, blocks, behind, st);
 }
 
 }  // namespace

@@ -12,8 +12,15 @@
 // The kernels of any type work in fp32 on split tf32 operands (tf32.cuh): a block of eight warps owns 32 rows and streams 64 of the
 // other side at a time, a warp has a 16 x 16 block of S1, S2 and G in its accumulators, turns them into dS1, dS2 (and P1 - lam P2)
 // there, and uses them as they are as operands of the gradients' products; a row's four warps add up their sums at the end.
-// They are bound by the ALU work of the operands' splitting.  At (1, 4 heads, 1000 tokens, 64 / 128, causal, fp32) dQ takes 125 us and
-// dK, dV 162; FMAs on 32 x 32 tiles took 296 and 530 (five 16-byte shared-memory reads for 16 multiply-adds of a thread).
+// They are bound by the latency of the splitting and of the products' chains, with 8 (dK, dV: 252 registers) or 16 (dQ) warps on an SM that
+// issue in 0.27 and 0.43 of the cycles.  Where there are few tiles, up to four blocks share one, each with every team-th tile of the other
+// side; their sums are added through distributed shared memory, in order.  At (1, 4 heads, 1000 tokens, 64 / 128, causal, fp32) dQ takes
+// 92 us and dK, dV 143; with one block for each tile, whose longest decides, 125 and 162; eight blocks 105 and 220; FMAs on 32 x 32 tiles
+// took 296 and 530 (five 16-byte shared-memory reads for 16 multiply-adds of a thread).
+#include <cooperative_groups.h>
+
+#include <algorithm>
+
 #include "diff.cuh"
 #include "tf32.cuh"
 
@@ -183,10 +190,18 @@ __device__ __forceinline__ void accumulate(float (&acc)[N][4], const float (&w)[
     }
   }
 }
-// The four warps of a row half hold sums over their own columns of the tiles: added up in shared memory, in order, and stored
+__device__ __forceinline__ void team_sync(int team) {
+  if (team > 1) cooperative_groups::this_cluster().sync();
+  else __syncthreads();
+}
+__device__ __forceinline__ float* of_member(float* p, int team, int member) {
+  return team > 1 ? cooperative_groups::this_cluster().map_shared_rank(p, member) : p;
+}
+// The four warps of a row half hold sums over their own columns of the tiles: added up in shared memory, in order, then over the blocks
+// that share the rows (`team` of them, a cluster), in order, and stored: a block of every kThreads-th elements
 template <typename T, int N>
 __device__ __forceinline__ void finish(float* buffer, const float (&acc)[N][4], int half, int part, T* dst, int64_t stride, int row0, int rows, int dim,
-                                       float f, int lane) {
+                                       float f, int lane, int team, int member) {
   constexpr int kPitch = 8 * N + 4;
   const int r = half * 16 + (lane >> 2), c = 2 * (lane & 3);
   for (int turn = 0; turn < 4; ++turn) {
@@ -200,17 +215,21 @@ __device__ __forceinline__ void finish(float* buffer, const float (&acc)[N][4], 
         *at = turn == 0 ? acc[n][e] : *at + acc[n][e];
       }
   }
-  __syncthreads();
-  for (int i = threadIdx.x; i < kOwn * 8 * N; i += kThreads) {
+  team_sync(team);
+  for (int i = threadIdx.x + member * kThreads; i < kOwn * 8 * N; i += kThreads * team) {
     const int row = i / (8 * N), col = i % (8 * N);
-    if (row0 + row < rows && col < dim) dst[(row0 + row) * stride + col] = from_f32<T>(buffer[row * kPitch + col] * f);
+    if (row0 + row >= rows || col >= dim) continue;
+    float x = 0.f;
+    for (int r = 0; r < team; ++r) x += *(of_member(buffer, team, r) + row * kPitch + col);
+    dst[(row0 + row) * stride + col] = from_f32<T>(x * f);
   }
+  team_sync(team);                                      // (others read this block's buffer)
 }
 
 // dQ1, dQ2 of 32 query rows of one head
 template <typename T, int DP>
-__global__ void __launch_bounds__(kThreads)
-diff_dq_any_kernel(const DiffParams p, const float* __restrict__ stats, int n_pad) {
+__global__ void __launch_bounds__(kThreads, DP == 64 ? 2 : 1)
+diff_dq_any_kernel(const DiffParams p, const float* __restrict__ stats, int n_pad, int team) {
   using Tile = AnyTile<DP>;
   constexpr int kPitch = Tile::kPitch, kVPitch = Tile::kVPitch;
   extern __shared__ __align__(16) float smem[];
@@ -218,7 +237,8 @@ diff_dq_any_kernel(const DiffParams p, const float* __restrict__ stats, int n_pa
   float* sg = sq + 2 * kOwn * kPitch;                   // [query][value dim]
   float* sk = sg + kOwn * kVPitch;                      // [map][key][dim]
   float* sv = sk + 2 * kStream * kPitch;                // [key][value dim]
-  const int h = blockIdx.y, b = blockIdx.z, g = h / (p.heads / p.kv_heads), q0 = (gridDim.x - 1 - blockIdx.x) * kOwn;
+  const int h = blockIdx.y, b = blockIdx.z, g = h / (p.heads / p.kv_heads), tiles = gridDim.x / team, member = blockIdx.x % team;
+  const int q0 = (tiles - 1 - static_cast<int>(blockIdx.x) / team) * kOwn;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, half = warp & 1, part = warp >> 1, shift = p.nk - p.nq;
   const int d8 = (p.head_dim + 7) / 8 * 8, v8 = (p.v_dim + 7) / 8 * 8;
   for (int m = 0; m < 2; ++m) tf32::Rows<T, kThreads, kOwn, DP>(p.q, b * p.qs.b + (2 * h + m) * p.qs.h, p.qs.r, p.nq, p.head_dim).load(sq + m * kOwn * kPitch, kPitch, q0);
@@ -239,7 +259,7 @@ diff_dq_any_kernel(const DiffParams p, const float* __restrict__ stats, int n_pa
   }
   float dq[2][DP / 8][4] = {}, dl = 0.f;
   const int end = p.causal ? min(p.nk, min(q0 + kOwn, p.nq) + shift) : p.nk;
-  for (int k0 = 0; k0 < end; k0 += kStream) {
+  for (int k0 = member * kStream; k0 < end; k0 += team * kStream) {
     __syncthreads();
     k1.load(sk, kPitch, k0);
     k2.load(sk + kStream * kPitch, kPitch, k0);
@@ -270,22 +290,23 @@ diff_dq_any_kernel(const DiffParams p, const float* __restrict__ stats, int n_pa
     for (int x = 16; x > 0; x >>= 1) dl += __shfl_xor_sync(0xffffffffu, dl, x);
     __shared__ float part_of[kThreads / 32];
     if (lane == 0) part_of[warp] = dl;
-    __syncthreads();
-    if (threadIdx.x == 0) {
+    team_sync(team);
+    if (threadIdx.x == 0 && member == 0) {
       dl = 0.f;
-      for (int x = 0; x < kThreads / 32; ++x) dl += part_of[x];
-      p.dlam_parts[(static_cast<int64_t>(b) * p.heads + h) * gridDim.x + q0 / kOwn] = dl;
+      for (int r = 0; r < team; ++r)
+        for (int x = 0; x < kThreads / 32; ++x) dl += *(of_member(part_of, team, r) + x);
+      p.dlam_parts[(static_cast<int64_t>(b) * p.heads + h) * tiles + q0 / kOwn] = dl;
     }
   }
 #pragma unroll
   for (int m = 0; m < 2; ++m)
-    finish<T>(smem, dq[m], half, part, static_cast<T*>(p.dq) + b * p.dqs.b + (2 * h + m) * p.dqs.h, p.dqs.r, q0, p.nq, p.head_dim, p.scale, lane);
+    finish<T>(smem, dq[m], half, part, static_cast<T*>(p.dq) + b * p.dqs.b + (2 * h + m) * p.dqs.h, p.dqs.r, q0, p.nq, p.head_dim, p.scale, lane, team, member);
 }
 
 // dK1, dK2, dV of 32 keys of one key head: over the query heads that share it, and their rows
 template <typename T, int DP>
 __global__ void __launch_bounds__(kThreads)
-diff_dkv_any_kernel(const DiffParams p, const float* __restrict__ stats, int n_pad) {
+diff_dkv_any_kernel(const DiffParams p, const float* __restrict__ stats, int n_pad, int team) {
   using Tile = AnyTile<DP>;
   constexpr int kPitch = Tile::kPitch, kVPitch = Tile::kVPitch;
   extern __shared__ __align__(16) float smem[];
@@ -293,7 +314,8 @@ diff_dkv_any_kernel(const DiffParams p, const float* __restrict__ stats, int n_p
   float* sv = sk + 2 * kOwn * kPitch;                   // [key][value dim]
   float* sq = sv + kOwn * kVPitch;                      // [map][query][dim]
   float* sg = sq + 2 * kStream * kPitch;                // [query][value dim]
-  const int g = blockIdx.y, b = blockIdx.z, group = p.heads / p.kv_heads, k0 = blockIdx.x * kOwn;
+  const int g = blockIdx.y, b = blockIdx.z, group = p.heads / p.kv_heads, member = blockIdx.x % team, k0 = static_cast<int>(blockIdx.x) / team * kOwn;
+  int turn = 0;                                         // of the members, tile by tile
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, half = warp & 1, part = warp >> 1, shift = p.nk - p.nq;
   const int d8 = (p.head_dim + 7) / 8 * 8, v8 = (p.v_dim + 7) / 8 * 8;
   for (int m = 0; m < 2; ++m) tf32::Rows<T, kThreads, kOwn, DP>(p.k, b * p.ks.b + (2 * g + m) * p.ks.h, p.ks.r, p.nk, p.head_dim).load(sk + m * kOwn * kPitch, kPitch, k0);
@@ -307,6 +329,9 @@ diff_dkv_any_kernel(const DiffParams p, const float* __restrict__ stats, int n_p
     const tf32::Rows<T, kThreads, kStream, DP> q1(p.q, b * p.qs.b + 2 * h * p.qs.h, p.qs.r, p.nq, p.head_dim), q2(p.q, b * p.qs.b + (2 * h + 1) * p.qs.h, p.qs.r, p.nq, p.head_dim);
     const tf32::Rows<T, kThreads, kStream, kValue> gr(p.dout, b * p.gs.b + h * p.gs.h, p.gs.r, p.nq, p.v_dim);
     for (int q0 = begin; q0 < p.nq; q0 += kStream) {
+      const bool mine = turn == member;
+      turn = turn + 1 == team ? 0 : turn + 1;
+      if (!mine) continue;
       __syncthreads();
       q1.load(sq, kPitch, q0);
       q2.load(sq + kStream * kPitch, kPitch, q0);
@@ -337,28 +362,43 @@ diff_dkv_any_kernel(const DiffParams p, const float* __restrict__ stats, int n_p
   }
 #pragma unroll
   for (int m = 0; m < 2; ++m)
-    finish<T>(smem, dk[m], half, part, static_cast<T*>(p.dk) + b * p.dks.b + (2 * g + m) * p.dks.h, p.dks.r, k0, p.nk, p.head_dim, p.scale, lane);
-  finish<T>(smem, dv, half, part, static_cast<T*>(p.dv) + b * p.dvs.b + g * p.dvs.h, p.dvs.r, k0, p.nk, p.v_dim, 1.f, lane);
+    finish<T>(smem, dk[m], half, part, static_cast<T*>(p.dk) + b * p.dks.b + (2 * g + m) * p.dks.h, p.dks.r, k0, p.nk, p.head_dim, p.scale, lane, team, member);
+  finish<T>(smem, dv, half, part, static_cast<T*>(p.dv) + b * p.dvs.b + g * p.dvs.h, p.dvs.r, k0, p.nk, p.v_dim, 1.f, lane, team, member);
+}
+
+// Blocks that share the rows of one tile, each with every team-th tile of the other side: as many as fill the SMs, and with a causal
+// mask even out rows of many and of few tiles.
+int team_of(int64_t blocks, int64_t streamed) {
+  int team = 1;
+  while (team < 4 && blocks * team < 4 * sm_count() && 2 * team <= cdiv64(streamed, kStream)) team *= 2;
+  return team;
+}
+
+template <typename Kernel>
+int launch_team(Kernel kernel, size_t smem, int team, int64_t tiles, int heads, int batch, cudaStream_t st, const DiffParams& p, const float* stats, int n_pad) {
+  const int rc = ensure_dynamic_smem(reinterpret_cast<const void*>(kernel), smem);
+  if (rc != ELSA_OK) return rc;
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeClusterDimension;
+  attr.val.clusterDim.x = static_cast<unsigned>(team); attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(static_cast<unsigned>(tiles * team), static_cast<unsigned>(heads), static_cast<unsigned>(batch));
+  cfg.blockDim = dim3(kThreads); cfg.dynamicSmemBytes = smem; cfg.stream = st;
+  cfg.attrs = &attr; cfg.numAttrs = team > 1 ? 1 : 0;
+  ELSA_CUDA_CHECK(cudaLaunchKernelEx(&cfg, kernel, p, stats, n_pad, team));
+  ELSA_LAUNCH_CHECK();
+  return ELSA_OK;
 }
 
 template <typename T, int DP>
 int any_t(const DiffParams& p, const float* stats, cudaStream_t st) {
   const int n_pad = static_cast<int>(align_up(p.nq, 128));
-  const auto dq = &diff_dq_any_kernel<T, DP>;
-  const auto dkv = &diff_dkv_any_kernel<T, DP>;
   constexpr int kSmem = AnyTile<DP>::kSmem;
-  int rc = ensure_dynamic_smem(reinterpret_cast<const void*>(dq), kSmem);
-  if (rc == ELSA_OK) rc = ensure_dynamic_smem(reinterpret_cast<const void*>(dkv), kSmem);
-  if (rc != ELSA_OK) return rc;
-  const dim3 qgrid(static_cast<unsigned>(cdiv64(p.nq, kOwn)), static_cast<unsigned>(p.heads), static_cast<unsigned>(p.batch));
-  dq<<<qgrid, kThreads, kSmem, st>>>(p, stats, n_pad);
-  ELSA_LAUNCH_CHECK();
-  if (p.nk > 0) {
-    const dim3 kgrid(static_cast<unsigned>(cdiv64(p.nk, kOwn)), static_cast<unsigned>(p.kv_heads), static_cast<unsigned>(p.batch));
-    dkv<<<kgrid, kThreads, kSmem, st>>>(p, stats, n_pad);
-    ELSA_LAUNCH_CHECK();
-  }
-  return ELSA_OK;
+  const int64_t q_tiles = cdiv64(p.nq, kOwn), k_tiles = cdiv64(p.nk, kOwn);
+  const int rc = launch_team(&diff_dq_any_kernel<T, DP>, kSmem, team_of(q_tiles * p.heads * p.batch, p.nk), q_tiles, p.heads, p.batch, st, p, stats, n_pad);
+  if (rc != ELSA_OK || p.nk == 0) return rc;
+  return launch_team(&diff_dkv_any_kernel<T, DP>, kSmem, team_of(k_tiles * p.kv_heads * p.batch, static_cast<int64_t>(p.nq) * (p.heads / p.kv_heads)), k_tiles,
+                     p.kv_heads, p.batch, st, p, stats, n_pad);
 }
 
 template <typename T>

@@ -1,8 +1,8 @@
 // fp32 products on the tensor cores' tf32 instruction (mma.sync m16n8k8, which reads the upper 19 bits of its operands): every operand x
 // is taken as hi + lo, hi = x cut to tf32's 11 significant bits and lo = x - hi (exact), rounded to as many, and a b = hi hi + hi lo +
 // lo hi.  lo is below 2^-10 of x, so an operand is right to 2^-21 of its size and what is left out, lo lo, is below 2^-20 of the
-// product and 2^-22 of it on average; sums are fp32.  (Both parts rounded would be better by a third and take 131 us where this takes
-// 125, for dQ at (1, 4 heads, 1000 tokens, 64 / 128, causal); cvt.rna, which runs at a fraction of the ALU's rate, 145.)  Three
+// product and 2^-22 of it on average; sums are fp32.  (Both parts rounded would be better by a third and take 5 % longer, for dQ
+// at (1, 4 heads, 1000 tokens, 64 / 128, causal); cvt.rna, which runs at a fraction of the ALU's rate, 16 %.)  Three
 // instructions of 1024 multiply-adds take the place of 32 FMAs of each thread and a quarter of their shared-memory reads.
 #pragma once
 

@@ -447,3 +447,16 @@ def test_training_with_more_sequences_than_the_tile_kernels_grid():
     for rows in (slice(0, 20), slice(32980, 33000)):
         _check_forward(out[rows], q[rows], k[rows], v[rows], lam)
         _check_gradients([g[rows] for g in got[:3]], q[rows], k[rows], v[rows], lam, dout[rows])
+
+
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("b", [20, 40])
+def test_gradients_with_tiles_of_one_two_and_four_blocks(b, causal):
+    """Blocks of the fp32 kernels share a tile while there are few tiles: 640 or 320 of queries, 400 or 200 of keys."""
+    q, k, v, lam = _inputs(b, 4, 2, 128, 150, 64, 128, torch.float32)
+    dout = _normal((b, 4, 128, 128), torch.float32, 20)
+    out, got = _run_train(q, k, v, lam, dout, is_causal=causal)
+    _check_forward(out, q, k, v, lam, causal=causal)
+    _check_gradients(got, q, k, v, lam, dout, causal)
+    assert all(torch.equal(x, y) for x, y in zip(got, _run_train(q, k, v, lam, dout, is_causal=causal)[1]))
+
