@@ -15,11 +15,12 @@
 //   merge_kernel       a warp per row, on the device early (it waits for the launch before it): 1 us less for a call.
 //
 // Measured, bf16, head dim 128: 256 x 8 caches of up to 2048 keys, 1.1 GB, 172 us = 6.3 TB/s, 0.96 of a plain copy's rate; 16 x 4
-// caches of up to 8192 keys of two maps (head dim 64, values of 128), 167 MB, 43 us: about 310 blocks of 960 keys in 296 places, 1.05
+// caches of up to 8192 keys of two maps (head dim 64, values of 128), 167 MB, 41 us: about 310 blocks of 960 keys in 296 places, 1.05
 // waves that take the time of two (33 to 46 us with 256 to 2048 keys a block, by chance).
 //
-// Softmax statistics, sums and O are fp32; P is rounded to the inputs' type for the second product (its error, half a step of
-// that type in each weight, averages out over the keys).  The reference max of a row moves only when it is exceeded by more than
+// Softmax statistics, sums and O are fp32.  P is rounded to the inputs' type for the second product: with up to 8 rows of a tile in two
+// parts, the second in the product's other rows; with more in one (its error, half a step of that type in each weight, averages out
+// over the keys; a second product for the rest took 55 us where the first alone takes 45).  The reference max of a row moves only when it is exceeded by more than
 // 2^8 (P <= 256 there), which saves most of the rescaling; any reference gives the same summary.
 #include <algorithm>
 
@@ -91,6 +92,12 @@ __device__ __forceinline__ void mma16816<__nv_bfloat16>(float (&d)[4], const uin
   asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
+// what rounding a and b to T (`rounded`) left of them, also in T
+template <typename T>
+__device__ __forceinline__ uint32_t rest2(float a, float b, uint32_t rounded) {
+  const T* e = reinterpret_cast<const T*>(&rounded);
+  return tc::pack2<T>(a - to_f32<T>(e[0]), b - to_f32<T>(e[1]));
+}
 __device__ __forceinline__ void ldsm_x4(uint32_t (&r)[4], uint32_t addr) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
 }
@@ -103,22 +110,26 @@ __device__ __forceinline__ void cp16(uint32_t dst, const void* src, int valid) {
 
 // DP, VP: head dim of q and k, and of v, rounded up to 64 or 128 (the columns beyond the real ones are zeros in shared memory,
 // written once).  Rows of a stage are an odd number of 16-byte pieces apart: the eight rows of an ldmatrix touch all 32 banks.
-template <int MAPS, int DP, int VP> struct MmaTile {
+// PAIRED: the tile has 8 rows, each twice: row r + 8 of P is what rounding row r to T left of it, so that the product has P to twice
+// the bits, at no cost, and the other 8 rows' exponentials are not there at all.
+template <int MAPS, int DP, int VP, bool PAIRED> struct MmaTile {
+  static constexpr int kRows = PAIRED ? kMmaRows / 2 : kMmaRows;
   static constexpr int kPitchK = (DP / 8 + 1) * 16, kPitchV = (VP / 8 + 1) * 16;
   static constexpr int kStage = kMmaKeys * (MAPS * kPitchK + kPitchV);
   static constexpr int kRing = kMmaWarps * kStages * kStage;
-  static constexpr int kMerge = kMmaWarps * MAPS * kMmaRows * (VP + 2) * 4;
+  static constexpr int kMerge = kMmaWarps * MAPS * kRows * (VP + 2) * 4;
   static constexpr int kSmem = kRing > kMerge ? kRing : kMerge;
 };
 
-template <typename T, int MAPS, int DP, int VP>
+template <typename T, int MAPS, int DP, int VP, bool PAIRED>
 __global__ void __launch_bounds__(kMmaThreads, 2)
 split_mma_kernel(const DecodeParams p) {
-  using Tile = MmaTile<MAPS, DP, VP>;
+  using Tile = MmaTile<MAPS, DP, VP, PAIRED>;
+  constexpr int kHalves = PAIRED ? 1 : 2;               // rows of a lane: qrow, and qrow + 8
   extern __shared__ __align__(16) uint8_t smem[];
   Block w;
   let_next_begin();
-  if (!locate(p, kMmaRows, w)) {
+  if (!locate(p, Tile::kRows, w)) {
     end_behind_previous();
     return;
   }
@@ -193,7 +204,7 @@ split_mma_kernel(const DecodeParams p) {
 #pragma unroll
   for (int half = 0; half < 2; ++half) {
     const int r = qrow + 8 * half;
-    const bool real = r < w.n_rows;
+    const bool real = half < kHalves && r < w.n_rows;
     lim[half] = real ? min(w.k1, row_limit(p, sg, w.len, w.row0 + r)) : w.k1;
 #pragma unroll
     for (int m = 0; m < MAPS; ++m) {
@@ -207,11 +218,11 @@ split_mma_kernel(const DecodeParams p) {
         }
     }
   }
-  float m_ref[MAPS][2], z[MAPS][2], o[MAPS][VP / 8][4];
+  float m_ref[MAPS][kHalves], z[MAPS][kHalves], o[MAPS][VP / 8][4];
 #pragma unroll
   for (int m = 0; m < MAPS; ++m) {
-    m_ref[m][0] = m_ref[m][1] = -CUDART_INF_F;
-    z[m][0] = z[m][1] = 0.f;
+#pragma unroll
+    for (int h = 0; h < kHalves; ++h) { m_ref[m][h] = -CUDART_INF_F; z[m][h] = 0.f; }
 #pragma unroll
     for (int n = 0; n < VP / 8; ++n)
 #pragma unroll
@@ -246,19 +257,19 @@ split_mma_kernel(const DecodeParams p) {
           for (int e = 0; e < 4; ++e)
             if (chunk0 + quad * 2 + n * 8 + (e & 1) >= lim[e >> 1]) s[n][e] = -CUDART_INF_F;
       }
-      float top[2];
-      bool move[2];
+      float top[kHalves];
+      bool move[kHalves];
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
+      for (int h = 0; h < kHalves; ++h) {
         top[h] = fmaxf(fmaxf(s[0][2 * h], s[0][2 * h + 1]), fmaxf(s[1][2 * h], s[1][2 * h + 1])) * c;
         top[h] = fmaxf(top[h], __shfl_xor_sync(0xffffffffu, top[h], 1));
         top[h] = fmaxf(top[h], __shfl_xor_sync(0xffffffffu, top[h], 2));
         move[h] = top[h] > m_ref[m][h] + kRescaleThreshold;
       }
-      if (__any_sync(0xffffffffu, move[0] || move[1])) {
-        float alpha[2];
+      if (__any_sync(0xffffffffu, move[0] || move[kHalves - 1])) {
+        float alpha[kHalves];
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
+        for (int h = 0; h < kHalves; ++h) {
           const float m_new = move[h] ? top[h] : m_ref[m][h];   // (a row's result does not depend on the rows beside it)
           alpha[h] = move[h] ? fast_exp2(m_ref[m][h] - m_new) : 1.f;
           m_ref[m][h] = m_new;
@@ -267,16 +278,20 @@ split_mma_kernel(const DecodeParams p) {
 #pragma unroll
         for (int n = 0; n < VP / 8; ++n)
 #pragma unroll
-          for (int e = 0; e < 4; ++e) o[m][n][e] *= alpha[e >> 1];
+          for (int e = 0; e < 4; ++e) o[m][n][e] *= alpha[PAIRED ? 0 : e >> 1];
       }
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
+      for (int h = 0; h < kHalves; ++h) {
         const float nm = m_ref[m][h] == -CUDART_INF_F ? 0.f : -m_ref[m][h];
         const float e0 = fast_exp2(fmaf(s[0][2 * h], c, nm)), e1 = fast_exp2(fmaf(s[0][2 * h + 1], c, nm));
         const float e2 = fast_exp2(fmaf(s[1][2 * h], c, nm)), e3 = fast_exp2(fmaf(s[1][2 * h + 1], c, nm));
         z[m][h] += (e0 + e1) + (e2 + e3);
         pf[m][h] = tc::pack2<T>(e0, e1);
         pf[m][2 + h] = tc::pack2<T>(e2, e3);
+        if (PAIRED) {
+          pf[m][1] = rest2<T>(e0, e1, pf[m][0]);
+          pf[m][3] = rest2<T>(e2, e3, pf[m][2]);
+        }
       }
     }
 #pragma unroll
@@ -295,17 +310,17 @@ split_mma_kernel(const DecodeParams p) {
 
   // [warp][map][row]: VP sums, then the max and the sum of weights
   float* merge = reinterpret_cast<float*>(smem);
-  auto slot = [&](int wp, int m, int r) { return merge + ((wp * MAPS + m) * kMmaRows + r) * (VP + 2); };
+  auto slot = [&](int wp, int m, int r) { return merge + ((wp * MAPS + m) * Tile::kRows + r) * (VP + 2); };
 #pragma unroll
   for (int m = 0; m < MAPS; ++m)
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
+    for (int h = 0; h < kHalves; ++h) {
       z[m][h] += __shfl_xor_sync(0xffffffffu, z[m][h], 1);
       z[m][h] += __shfl_xor_sync(0xffffffffu, z[m][h], 2);
       if (qrow + 8 * h >= w.n_rows) continue;
       float* dst = slot(warp, m, qrow + 8 * h);
 #pragma unroll
-      for (int n = 0; n < VP / 8; ++n) *reinterpret_cast<float2*>(dst + n * 8 + quad * 2) = make_float2(o[m][n][2 * h], o[m][n][2 * h + 1]);
+      for (int n = 0; n < VP / 8; ++n) *reinterpret_cast<float2*>(dst + n * 8 + quad * 2) = PAIRED ? make_float2(o[m][n][0] + o[m][n][2], o[m][n][1] + o[m][n][3]) : make_float2(o[m][n][2 * h], o[m][n][2 * h + 1]);
       if (quad == 0) *reinterpret_cast<float2*>(dst + VP) = make_float2(m_ref[m][h], z[m][h]);
     }
   __syncthreads();
@@ -615,17 +630,18 @@ merge_kernel(const DecodeParams p, int n_parts) {
 }
 
 template <typename T, int MAPS, int DP, int VP>
-int launch_mma(const DecodeParams& p, int64_t blocks, bool behind, cudaStream_t st) {
-  const auto kernel = &split_mma_kernel<T, MAPS, DP, VP>;
-  const int rc = ensure_dynamic_smem(reinterpret_cast<const void*>(kernel), MmaTile<MAPS, DP, VP>::kSmem);
+int launch_mma(const DecodeParams& p, int64_t blocks, bool paired, bool behind, cudaStream_t st) {
+  const auto kernel = paired ? &split_mma_kernel<T, MAPS, DP, VP, true> : &split_mma_kernel<T, MAPS, DP, VP, false>;
+  const int smem = paired ? MmaTile<MAPS, DP, VP, true>::kSmem : MmaTile<MAPS, DP, VP, false>::kSmem;
+  const int rc = ensure_dynamic_smem(reinterpret_cast<const void*>(kernel), smem);
   if (rc != ELSA_OK) return rc;
-  return launch_behind(behind, kernel, static_cast<unsigned>(blocks), kMmaThreads, MmaTile<MAPS, DP, VP>::kSmem, st, p);
+  return launch_behind(behind, kernel, static_cast<unsigned>(blocks), kMmaThreads, smem, st, p);
 }
 
 template <typename T>
-int launch_mma_t(const DecodeParams& p, int64_t blocks, bool behind, cudaStream_t st) {
-  if (p.maps == 2) return p.v_dim > 64 ? launch_mma<T, 2, 64, 128>(p, blocks, behind, st) : launch_mma<T, 2, 64, 64>(p, blocks, behind, st);
-  return p.head_dim > 64 || p.v_dim > 64 ? launch_mma<T, 1, 128, 128>(p, blocks, behind, st) : launch_mma<T, 1, 64, 64>(p, blocks, behind, st);
+int launch_mma_t(const DecodeParams& p, int64_t blocks, bool paired, bool behind, cudaStream_t st) {
+  if (p.maps == 2) return p.v_dim > 64 ? launch_mma<T, 2, 64, 128>(p, blocks, paired, behind, st) : launch_mma<T, 2, 64, 64>(p, blocks, paired, behind, st);
+  return p.head_dim > 64 || p.v_dim > 64 ? launch_mma<T, 1, 128, 128>(p, blocks, paired, behind, st) : launch_mma<T, 1, 64, 64>(p, blocks, paired, behind, st);
 }
 
 template <typename T, int MAPS, int DP, int VP>
@@ -661,8 +677,11 @@ bool decode_mma_ok(const DecodeParams& p, int dtype) {
 int decode_split(DecodeParams& p, int dtype, bool behind, cudaStream_t st) {
   if (p.head_dim > kAnyDim || p.v_dim > kAnyDim) return ELSA_ERR_UNSUPPORTED;
   const bool mma = decode_mma_ok(p, dtype);
-  const int tile = mma ? kMmaRows : kAnyRows;
   const int rows_b = p.heads / p.kv_heads * p.nq;
+  // (a shared cache is for the rows of all sequences: with more than 8 of them, tiles of 8 would read it twice as often)
+  bool paired = mma && rows_b <= kMmaRows / 2;
+  for (int i = 0; i < p.n_segs; ++i) paired = paired && (!p.seg[i].shared || decode_rows(p) <= kMmaRows / 2);
+  const int tile = paired ? kMmaRows / 2 : mma ? kMmaRows : kAnyRows;
   int64_t blocks = 0;
   for (int i = 0; i < p.n_segs; ++i) {
     DecodeSegment& s = p.seg[i];
@@ -672,7 +691,7 @@ int decode_split(DecodeParams& p, int dtype, bool behind, cudaStream_t st) {
   }
   if (blocks == 0) return ELSA_OK;
   if (blocks > 0x7fffffffll) return ELSA_ERR_UNSUPPORTED;
-  if (mma) return dtype == ELSA_F16 ? launch_mma_t<__half>(p, blocks, behind, st) : launch_mma_t<__nv_bfloat16>(p, blocks, behind, st);
+  if (mma) return dtype == ELSA_F16 ? launch_mma_t<__half>(p, blocks, paired, behind, st) : launch_mma_t<__nv_bfloat16>(p, blocks, paired, behind, st);
   if (dtype == ELSA_F32) return launch_any_t<float>(p, blocks, behind, st);
   return dtype == ELSA_F16 ? launch_any_t<__half>(p, blocks, behind, st) : launch_any_t<__nv_bfloat16>(p, blocks, behind, st);
 }
