@@ -1,5 +1,5 @@
 // Differential attention, backward, on the 5th-generation tensor cores (fp16 / bf16, head dim <= 64, value dim <= 128, multiples of 8).
-// The formulas are in diff_any.cu.  Nine products for each pair of tiles, G = g V^T shared by the two maps, no atomics:
+// The formulas are in diff_any.cu.  Eleven products for each pair of tiles, G = g V^T shared by the two maps, no atomics:
 //
 //   dq body    one CTA per 128 query rows of an output head, 64-key tiles streamed through a 4-stage ring:
 //                S1 = Q1 K1^T, S2 = Q2 K2^T, G = g V^T                                (N = 64)
@@ -20,6 +20,10 @@
 //
 // Both bodies: 16 fold warps (four threads per row, 16 columns each), a TMA producer warp, an MMA-issuing warp; all waits bounded.
 // P, dS and P1 - lam P2 are rounded to the inputs' type for the second products; statistics and sums are fp32.
+//
+// Measured, (2, 8 heads, 8192 tokens, 64 / 128) causal bf16: 1040 to 1100 us under the power cap, 900 TFLOP/s of its eleven products; 1200 before the folds
+// took pairs (fma.f32x2).  A tile takes 1670 cycles in the dq body and 2090 in the dkv body: the products that read both operands from shared
+// memory, and the folds, 54 % of the ex2 unit.  A part of the exponentials on the FMA pipe (every 2nd, 4th or 8th pair): 1100 to 1180.
 #include <algorithm>
 #include <type_traits>
 

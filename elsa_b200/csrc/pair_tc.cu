@@ -15,7 +15,9 @@
 // fold holds S_t(j) in registers and runs during the exponentials of tile j; a fold warp waits for the tensor pipe only when its
 // maximum moves.  Measured, (2, 8, 8192, 64 / 128) causal bf16: 128-key tiles, whose P has no columns of its own, so that scores,
 // exponentials and P V of a chain follow one another, 460 us; 64-key tiles with two S_t, P over the scores it comes from, 460 (the
-// scores of tile j + 1 wait for P V of tile j - 1); the latter with the next scores read ahead of the exponentials 550.
+// scores of tile j + 1 wait for P V of tile j - 1); the latter with the next scores read ahead of the exponentials 550;
+// this form 460 to 490 by the card and its clock (1.75 GHz under the power cap).  Rows128: 0.72 us a tile with few CTAs on the card, 0.9 with
+// all of them, and about 14 us of a CTA besides its tiles.
 //
 // Bound: the ex2 unit, 2 x 128 x 64 exponentials for each tile (1024 cycles; the tensor pipe, limited by its shared-memory operands,
 // needs 900 for Diff and 1280 for Rows128).

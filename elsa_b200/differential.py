@@ -1,5 +1,5 @@
 """Differential attention: the difference of two softmax maps with a learned weight, over one set of values -- forward, backward, and the
-form for single tokens over a key cache (csrc/diff_tc.cu, csrc/diff_bwd_tc.cu, csrc/diff_any.cu, csrc/decode.cu).
+form for single tokens over a key cache (csrc/pair_tc.cu, csrc/diff_bwd_tc.cu, csrc/diff_any.cu, csrc/decode.cu).
 
 The reference has no counterpart; names and checks follow `twopass_attention` and `twopass_attention_train`.
 """

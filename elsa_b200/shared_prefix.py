@@ -1,6 +1,6 @@
 """Attention of a batch whose sequences share a long prefix (a system prompt, a document, the samples of one prompt): the serving
 form of the two-pass scheme, in which the prefix and each sequence's own cache give (m, z, s) summaries that one merge joins
-(csrc/decode.cu, csrc/fold_tc.cu, csrc/fold_tcw.cu).
+(csrc/pair_tc.cu, csrc/decode.cu).
 
 The reference has no counterpart; names and checks follow `twopass_attention`.
 """
