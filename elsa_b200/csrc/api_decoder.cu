@@ -66,12 +66,13 @@ int plan_prefix(int dtype, int batch, int heads, int kv_heads, int nq, int head_
   }
   if (pl->tiles) {
     // One CTA for each 256 rows, key head and part, one CTA on an SM: waves x (64-key tiles of a part + what a CTA costs besides, about
-    // 18 of them).  The split kernel of the sequences' own keys runs beside it, on the SMs that it leaves free: about 0.7 of them read at
-    // full speed, fewer in proportion.  So few parts may be the best, a prefix that takes long on some SMs while the caches stream
-    // through the others.  Measured (head dim 128, bf16): 256 sequences with 2048 keys behind 32768, 32 CTAs a part: 252 us with 2 parts,
-    // 271 with 3, 306 with 9 (two full waves, then the caches; under the power cap of a long run 307, 312, 336); 64 with 1024 behind 8192, 8 CTAs a part: 56 us with 7 parts, 69
-    // with 4, 67 with 18; 24 x 3 with 333 behind 4097, 6 CTAs a part: 29.7 us with 13, 33.8 with 17, 35.9 with 22.  (With caches all but
-    // empty the first of these loses, 241 us against 198 one after the other; half full it is 247 against 280, full 335 against 386.)
+    // 13 of them).  The split kernel of the sequences' own keys runs beside it, on the SMs that it leaves free: 0.8 of them read at full
+    // speed, fewer in proportion.  So few parts may be the best, a prefix that takes long on some SMs while the caches stream through
+    // the others.  Measured, us a call in a long run: 256 sequences with up to 2048 keys behind 32768 (8 heads of 128), 32 CTAs a part:
+    // 288 with 2 parts, 294 with 3, 317 with 9 (two full waves, then the caches); 64 with up to 1024 behind 8192, 8 CTAs a part: 44.2 with
+    // 5, 50 with 4, 46 with 7, 59 with 17; 24 with up to 333 behind 4097 (3 heads of 96, five tokens), 6 CTAs a part: 22.5 with 8 to 11,
+    // 24.6 with 5, 26.7 with 17.  (With caches all but empty the first of these loses, 241 us against 198 one after the other; half full it
+    // is 247 against 280, full 335 against 386.)
     const double tile_us = 0.8, bytes_us = 6.3e6;
     const double own = n_own > 0 ? (2.0 * head_dim * batch * kv_heads * n_own / bytes_us + 9.0) / tile_us : 0.0;    // in tiles too, of caches half full
     const int64_t ctas = cdiv64(rows, 256) * kv_heads, tiles = cdiv64(n_prefix, 64), sms = sm_count();
@@ -79,8 +80,8 @@ int plan_prefix(int dtype, int batch, int heads, int kv_heads, int nq, int head_
     double best_cost = 0.0;
     for (int64_t parts = 1; parts <= std::min<int64_t>(tiles, 64); ++parts) {
       const int64_t per = cdiv64(tiles, parts), all = ctas * cdiv64(tiles, per);
-      const double prefix = static_cast<double>(cdiv64(all, sms) * (per + 18));
-      const double beside = prefix * std::min(1.0, std::max<int64_t>(0, sms - all) / (0.7 * sms));    // of the caches, while the prefix takes its time
+      const double prefix = static_cast<double>(cdiv64(all, sms) * (per + 13));
+      const double beside = prefix * std::min(1.0, std::max<int64_t>(0, sms - all) / (0.8 * sms));    // of the caches, meanwhile
       const double cost = prefix + std::max(0.0, own - beside);
       if (best == 0 || cost < best_cost) { best = per; best_cost = cost; }
     }

@@ -9,8 +9,7 @@
 //                      with running max, sum and O in registers; the four are merged through shared memory at the end.  mma.sync
 //                      and not tcgen05: a tile has 16 rows here and not 128, a warp's products stay in its registers, and 8
 //                      bytes are loaded for every row's multiply-add that either could do.
-//                      A warp needs about 2300 cycles for 16 keys, a chain of products, shuffles and exponentials: with eight warps an
-//                      SM reads 52 GB/s, and about 0.7 of the SMs are enough for the memory's rate.
+//                      A warp needs about 2300 cycles for 16 keys, a chain of products, shuffles and exponentials.
 //   split_any_kernel   any type, any head dim up to 128, any stride, in fp32 (split tf32 operands) on 32 x 32 tiles.
 //   merge_kernel       a warp per row, on the device early (it waits for the launch before it): 1 us less for a call.
 //

@@ -17,7 +17,7 @@
 // exponentials and P V of a chain follow one another, 460 us; 64-key tiles with two S_t, P over the scores it comes from, 460 (the
 // scores of tile j + 1 wait for P V of tile j - 1); the latter with the next scores read ahead of the exponentials 550;
 // this form 460 to 490 by the card and its clock (1.75 GHz under the power cap).  Rows128: 0.72 us a tile with few CTAs on the card, 0.9 with
-// all of them, and about 14 us of a CTA besides its tiles.
+// all of them, and about 10 us of a CTA besides its tiles (14 when each thread fetched its own query row and wrote its own row of sums).
 //
 // Bound: the ex2 unit, 2 x 128 x 64 exponentials for each tile (1024 cycles; the tensor pipe, limited by its shared-memory operands,
 // needs 900 for Diff and 1280 for Rows128).
@@ -25,8 +25,8 @@
 // The reference max of a row moves only when it is exceeded by more than 2^8; a row's result does not depend on the rows beside it.
 // P is rounded to the inputs' type (its error, half a step in each weight, averages out over the keys); sums and statistics are fp32.
 // Diff: each map is normalised by its own sum at the end; lam O_1 / z_1 goes through shared memory to the threads that hold the same rows
-// of O_0.  Rows: a thread gathers its own query row into the swizzled operand (rows of a kv head are not evenly spaced in q) and writes
-// its row's summary.
+// of O_0.  Rows: a warp gathers its query rows into the swizzled operand (rows of a kv head are not evenly spaced in q) and writes its rows'
+// summaries through shared memory.
 #include <type_traits>
 
 #include "pair_tc.cuh"
@@ -236,20 +236,26 @@ pair_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant__ 
     const uint32_t lane_off = static_cast<uint32_t>((warp & 3) * 32) << 16;
     const float c = MODE == kDiff ? p.scale_log2 : rp.scale_log2;
     if constexpr (MODE != kDiff) {
-      // this thread's query row into the operand tile: 16-byte piece x of row r of a 64-column half at piece x ^ (r & 7)
+      // this warp's query rows into the operand tile: 16-byte piece x of row r of a 64-column half at piece x ^ (r & 7).  A lane finds its own
+      // row's place in q; then 8 or 16 lanes fetch a row together.
       const int rows = static_cast<int>(decode_rows(rp)), pieces = rp.head_dim / 8;
-      const uint4* src = nullptr;
+      unsigned long long src = 0;
       if (qi < rows) {
         const int per = prm.group * rp.nq, b = qi / per, r = qi - b * per, h = r / rp.nq, i = r - h * rp.nq;
-        src = reinterpret_cast<const uint4*>(static_cast<const T*>(rp.q) + b * rp.qs.b + static_cast<int64_t>(gi * prm.group + h) * rp.qs.h + i * rp.qs.r);
+        src = reinterpret_cast<unsigned long long>(static_cast<const T*>(rp.q) + b * rp.qs.b + static_cast<int64_t>(gi * prm.group + h) * rp.qs.h + i * rp.qs.r);
       }
-      uint4 v[8];
+      constexpr int kLanes = 8 * Sh::kQHalves, kPass = 32 / kLanes;      // lanes of a row, rows of one access
+      const int piece = lane % kLanes;
+      uint4 v[kLanes];
 #pragma unroll
-      for (int h = 0; h < Sh::kQHalves; ++h) {
+      for (int x = 0; x < kLanes; ++x) {
+        const unsigned long long at = __shfl_sync(0xffffffffu, src, x * kPass + lane / kLanes);
+        v[x] = at && piece < pieces ? reinterpret_cast<const uint4*>(at)[piece] : make_uint4(0, 0, 0, 0);
+      }
 #pragma unroll
-        for (int x = 0; x < 8; ++x) v[x] = src && 8 * h + x < pieces ? src[8 * h + x] : make_uint4(0, 0, 0, 0);
-#pragma unroll
-        for (int x = 0; x < 8; ++x) *reinterpret_cast<uint4*>(smem_gen + q_off(t, h) + row * 128 + ((x ^ (row & 7)) << 4)) = v[x];
+      for (int x = 0; x < kLanes; ++x) {
+        const int r = (warp & 3) * 32 + x * kPass + lane / kLanes;
+        *reinterpret_cast<uint4*>(smem_gen + q_off(t, piece / 8) + r * 128 + ((piece % 8 ^ (r & 7)) << 4)) = v[x];
       }
       fence_proxy_async_smem();
       mbar_arrive_warp(bar_q, lane);
@@ -386,15 +392,26 @@ pair_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant__ 
         rp.m[ro] = zsum != 0.f ? m_ref : -CUDART_INF_F;
         rp.z[ro] = zsum;
       }
+      // The warp's 32 rows of sums stand side by side in memory: through shared memory (over the ring, which neither chain reads any more),
+      // so that whole lines are written.
+      if (alive && n_t > 0) alive = mbar_wait_warp(bar_o(1 - t), 0, &abort_flag, prm.status, BAR_O);
+      constexpr int kPitch = 64 * Sh::kVSlots + 4;         // (rows 16 bytes apart in the banks)
+      float* buffer = reinterpret_cast<float*>(smem_gen + 2 * Sh::kQHalves * kTileBytes) + warp * 32 * kPitch;
       for (int h = 0; h < 2 * v_halves; ++h) {
-        float o[32];
         uint32_t r[32];
         tmem_ld32(tO(t) + lane_off + 32 * h, r);
         tmem_wait_ld();
+        if (alive) {
 #pragma unroll
-        for (int i = 0; i < 32; ++i) o[i] = __uint_as_float(r[i]);
-        if (row_ok) store32<float>(rp.s + ro * v_dim + 32 * h, o, v_dim - 32 * h);
+          for (int i = 0; i < 32; i += 4)
+            *reinterpret_cast<uint4*>(buffer + lane * kPitch + 32 * h + i) = make_uint4(r[i], r[i + 1], r[i + 2], r[i + 3]);
+        }
       }
+      __syncwarp();
+      const int vecs = v_dim / 4, first = qi - lane, n_vecs = alive ? min(32, rows - first) * vecs : 0;
+      float4* dst = reinterpret_cast<float4*>(rp.s + (ro - lane) * v_dim);
+#pragma unroll 1
+      for (int i = lane; i < n_vecs; i += 32) dst[i] = *reinterpret_cast<const float4*>(buffer + i / vecs * kPitch + i % vecs * 4);
     }
   }
 
