@@ -153,3 +153,70 @@ def test_rotary_positions_are_refused_for_swin_windows():
     from tests.standins import SwinWindowAttention
     with pytest.raises(ValueError, match="rotary"):
         E.patch_timm_attention(torch.nn.Sequential(SwinWindowAttention(32, 2, (7, 7))), elsa_kwargs={"rotary": E.Rotary(E.rotary_frequencies(16)[0])})
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.float32])
+def test_rows_whose_offsets_pass_32_bits(dtype):
+    """Rows 2^23 elements apart: the last ones begin behind element 2^31."""
+    n, step = 300, 2 ** 23
+    pool = torch.empty(n * step, dtype=dtype, device="cuda")
+
+    def spread(t, at):
+        view = pool[at:].as_strided(t.shape, (t.shape[1] * t.shape[3], t.shape[3], step, 1))
+        return view.copy_(t)
+
+    gen = torch.Generator().manual_seed(5)
+    q, k, v, dout = (torch.randn(shape, generator=gen).to(dtype).cuda() for shape in ((1, 4, n, 64), (1, 2, n, 64), (1, 1, n, 128), (1, 2, n, 128)))
+    far = [spread(t, 1024 * i) for i, t in enumerate((q, k, v, dout))]
+    assert far[0][0, 0, -1].data_ptr() - pool.data_ptr() > 2 ** 31 * pool.element_size()
+    f, lam = E.rotary_frequencies(64, device="cuda")[0], torch.tensor([0.3, 0.6], device="cuda")
+    for got, want in zip(E.rotary_embedding(far[0], far[1], f), E.rotary_embedding(q, k, f)):
+        assert torch.equal(got, want)
+    for nq in (1, n):                       # the decoding form and the tiles
+        assert torch.equal(E.differential_attention(far[0][:, :, n - nq:], far[1], far[2], lam, is_causal=True),
+                           E.differential_attention(q[:, :, n - nq:].contiguous(), k, v, lam, is_causal=True))
+    grads = []
+    for args, g in (((q, k, v), dout), (far[:3], far[3])):
+        leaves = [t.detach().requires_grad_(True) for t in args]
+        grads.append(torch.autograd.grad(E.differential_attention_train(*leaves, lam, is_causal=True), leaves, g))
+    assert all(torch.equal(a, b) for a, b in zip(*grads))
+    # the prefix's rows for many and for few queries, the own caches beside it
+    for b in (1, 40):
+        qs = torch.randn((b, 4, 1, 64), generator=gen).to(dtype).cuda()
+        own = torch.randn((b, 2, 50, 64), generator=gen).to(dtype).cuda()
+        assert torch.equal(E.shared_prefix_attention(qs, far[1][0], far[1][0], own, own), E.shared_prefix_attention(qs, k[0], k[0], own, own))
+
+
+def test_calls_from_several_threads():
+    import threading
+    gen = torch.Generator().manual_seed(9)
+    q, k, v = (torch.randn(shape, generator=gen).half().cuda() for shape in ((2, 4, 200, 64), (2, 2, 200, 64), (2, 1, 200, 128)))
+    f, lam = E.rotary_frequencies(64, device="cuda")[0], torch.tensor([0.3, 0.6], device="cuda")
+    qs, own = (torch.randn(shape, generator=gen).half().cuda() for shape in ((40, 4, 1, 64), (40, 2, 50, 64)))
+
+    def step():
+        leaves = [t.detach().requires_grad_(True) for t in (q, k, v)]
+        turned = E.rotary_embedding(leaves[0], leaves[1], f)
+        out = E.differential_attention_train(*turned, leaves[2], lam, is_causal=True)
+        return [out.detach(), *torch.autograd.grad(out, leaves, v.repeat(1, 2, 1, 1)), E.shared_prefix_attention(qs, k[0], k[0], own, own),
+                E.differential_attention(q[:, :, :1], k, v, lam)]
+
+    want = step()
+    torch.cuda.synchronize()
+    failures = []
+
+    def work():
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for _ in range(20):
+                got = step()
+                torch.cuda.current_stream().synchronize()
+                if not all(torch.equal(a, b) for a, b in zip(got, want)):
+                    failures.append(threading.get_ident())
+
+    threads = [threading.Thread(target=work) for _ in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not failures
+
