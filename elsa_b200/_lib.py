@@ -65,6 +65,7 @@ SIGNATURES = {
     "elsa_shared_prefix_workspace_bytes": (c_int64, [c_int] * 8),
     "elsa_shared_prefix_attention": (c_int, [_P] * 9 + [c_int64] + [c_int] * 8 + [c_double, _P]),
     "elsa_differential_workspace_bytes": (c_int64, [c_int] * 8),
+    "elsa_differential_workspace_bytes_for": (c_int64, [_P] * 6 + [c_int] * 8),
     "elsa_differential_forward": (c_int, [_P] * 4 + [c_int, c_int] + [_P] * 6 + [c_int64] + [c_int] * 9 + [c_double, _P]),
     "elsa_differential_backward_workspace_bytes": (c_int64, [c_int] * 8),
     "elsa_differential_backward": (c_int, [_P] * 4 + [c_int, c_int] + [_P] * 10 + [c_int64] + [c_int] * 9 + [c_double, _P]),
@@ -94,7 +95,7 @@ def load():
 _HOST_ENTRIES = ("elsa_forward_workspace_bytes", "elsa_twopass_forward", "elsa_twopass_forward_strided",
                  "elsa_backward_workspace_bytes", "elsa_twopass_backward", "elsa_twopass_backward_strided", "elsa_strerror",
                  "elsa_last_cuda_error", "elsa_rotary", "elsa_shared_prefix_workspace_bytes", "elsa_shared_prefix_attention",
-                 "elsa_differential_workspace_bytes", "elsa_differential_forward", "elsa_differential_backward_workspace_bytes",
+                 "elsa_differential_workspace_bytes_for", "elsa_differential_forward", "elsa_differential_backward_workspace_bytes",
                  "elsa_differential_backward")
 _host_module = None
 _host_tried = False

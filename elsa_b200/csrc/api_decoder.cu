@@ -140,6 +140,12 @@ bool diff_inputs_in_tiles(const DiffParams& p) {
          (p.nk == 0 || (diff_rows_ok(p.k, p.ks, p.head_dim, 2 * p.kv_heads, p.batch) && diff_rows_ok(p.v, p.vs, p.v_dim, p.kv_heads, p.batch)));
 }
 
+// whether the forward runs on the tile kernel, which needs no workspace
+// (what stands behind a sequence's last key must not be read: the tile kernel's loads are bounded by the tensors only)
+bool diff_forward_in_tiles(const DiffPlan& pl, const DiffParams& p, const int* lengths) {
+  return pl.tensor_tiles && !lengths && diff_inputs_in_tiles(p) && diff_rows_ok(p.out, p.os, p.v_dim, p.heads, p.batch);
+}
+
 }  // namespace
 
 extern "C" int elsa_rotary(const void* q, void* q_out, const int64_t* q_strides, int q_heads, const void* k, void* k_out,
@@ -215,6 +221,16 @@ extern "C" int64_t elsa_differential_workspace_bytes(int dtype, int batch, int h
   return plan_diff(dtype, batch, heads, kv_heads, nq, nk, head_dim, v_dim, &pl) == ELSA_OK ? pl.bytes() : -1;
 }
 
+extern "C" int64_t elsa_differential_workspace_bytes_for(const void* q, const void* k, const void* v, const int* lengths, const void* out,
+                                                         const int64_t* strides, int dtype, int batch, int heads, int kv_heads, int nq, int nk,
+                                                         int head_dim, int v_dim) {
+  DiffPlan pl;
+  if (plan_diff(dtype, batch, heads, kv_heads, nq, nk, head_dim, v_dim, &pl) != ELSA_OK || !strides) return -1;
+  DiffParams d = diff_params(q, k, v, nullptr, 0, 0, strides, batch, heads, kv_heads, nq, nk, head_dim, v_dim, 0, 1.0);
+  d.out = const_cast<void*>(out); d.os = Strides{strides[9], strides[10], strides[11]};
+  return diff_forward_in_tiles(pl, d, lengths) ? 0 : pl.bytes();
+}
+
 extern "C" int elsa_differential_forward(const void* q, const void* k, const void* v, const void* lam, int lam_dtype, int lam_stride,
                                          const int* lengths, void* out, const int64_t* strides, void* out2, float* lse, void* workspace,
                                          int64_t workspace_bytes, int dtype, int batch, int heads, int kv_heads, int nq, int nk,
@@ -223,16 +239,15 @@ extern "C" int elsa_differential_forward(const void* q, const void* k, const voi
   int rc = plan_diff(dtype, batch, heads, kv_heads, nq, nk, head_dim, v_dim, &pl);
   if (rc != ELSA_OK) return rc;
   if (!q || !lam || !out || !strides || (nk > 0 && (!k || !v)) || !dtype_ok(lam_dtype) || !scale_ok(scale)) return ELSA_ERR_INVALID_ARGUMENT;
-  if (pl.bytes() > 0 && (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 255u) || workspace_bytes < pl.bytes())) return ELSA_ERR_WORKSPACE;
   auto st = static_cast<cudaStream_t>(stream);
   DiffParams d = diff_params(q, k, v, lam, lam_dtype, lam_stride, strides, batch, heads, kv_heads, nq, nk, head_dim, v_dim, is_causal, scale);
   d.out = out; d.os = Strides{strides[9], strides[10], strides[11]};
   d.out2 = out2; d.lse = lse;
-  // (what stands behind a sequence's last key must not be read: the tile kernel's loads are bounded by the tensors only)
-  if (pl.tensor_tiles && !lengths && diff_inputs_in_tiles(d) && diff_rows_ok(out, d.os, v_dim, heads, batch)) {
+  if (diff_forward_in_tiles(pl, d, lengths)) {
     if ((rc = device_status_ok()) != ELSA_OK) return rc;
     return diff_tc_fwd(d, dtype, st);
   }
+  if (pl.bytes() > 0 && (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 255u) || workspace_bytes < pl.bytes())) return ELSA_ERR_WORKSPACE;
   DecodeParams p{};
   p.q = q; p.qs = d.qs;
   p.batch = batch; p.heads = heads; p.kv_heads = kv_heads; p.nq = nq; p.head_dim = head_dim; p.v_dim = v_dim; p.maps = 2;

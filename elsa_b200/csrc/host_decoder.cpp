@@ -24,7 +24,7 @@ using torch::autograd::variable_list;
 decltype(&elsa_rotary) f_rotary = nullptr;
 decltype(&elsa_shared_prefix_workspace_bytes) f_prefix_ws = nullptr;
 decltype(&elsa_shared_prefix_attention) f_prefix = nullptr;
-decltype(&elsa_differential_workspace_bytes) f_diff_ws = nullptr;
+decltype(&elsa_differential_workspace_bytes_for) f_diff_ws = nullptr;
 decltype(&elsa_differential_forward) f_diff = nullptr;
 decltype(&elsa_differential_backward_workspace_bytes) f_diff_bwd_ws = nullptr;
 decltype(&elsa_differential_backward) f_diff_bwd = nullptr;
@@ -286,14 +286,15 @@ at::Tensor diff_forward(const at::Tensor& q, const at::Tensor& k, const at::Tens
   at::Tensor out = new_like(q, st, c.batch, c.heads, c.nq, c.dv);
   row_strides(out, st + 9);
   c10::cuda::CUDAGuard guard(q.device());
-  const int64_t need = f_diff_ws(c.dt, c.batch, c.heads, c.kv_heads, c.nq, c.nk, c.d, c.dv);
-  TORCH_CHECK_VALUE(need >= 0, "elsa_b200: unsupported problem size for differential_attention");
-  const int64_t bytes = std::max<int64_t>(need, 256);
-  c10::DataPtr ws = workspace(bytes);
+  const int* n = lengths.defined() ? lengths.const_data_ptr<int>() : nullptr;
+  const int64_t bytes = f_diff_ws(data_of(q), data_of(k), data_of(v), n, data_of(out), st, c.dt, c.batch, c.heads, c.kv_heads, c.nq, c.nk, c.d, c.dv);
+  TORCH_CHECK_VALUE(bytes >= 0, "elsa_b200: unsupported problem size for differential_attention");
+  c10::DataPtr ws;                                      // (the tiles need none)
+  if (bytes > 0) ws = workspace(bytes);
   const Lam l = lam_of(lam);
-  check_status(f_diff(data_of(q), data_of(k), data_of(v), l.p, l.dtype, l.stride, lengths.defined() ? lengths.const_data_ptr<int>() : nullptr, data_of(out), st,
-                      out2.defined() ? data_of(out2) : nullptr, lse.defined() ? lse.mutable_data_ptr<float>() : nullptr, ws.get(), bytes, c.dt, c.batch,
-                      c.heads, c.kv_heads, c.nq, c.nk, c.d, c.dv, c.causal, c.scale, stream_of(q.device())),
+  check_status(f_diff(data_of(q), data_of(k), data_of(v), l.p, l.dtype, l.stride, n, data_of(out), st, out2.defined() ? data_of(out2) : nullptr,
+                      lse.defined() ? lse.mutable_data_ptr<float>() : nullptr, ws.get(), bytes, c.dt, c.batch, c.heads, c.kv_heads, c.nq, c.nk, c.d, c.dv,
+                      c.causal, c.scale, stream_of(q.device())),
                "elsa_differential_forward");
   return out;
 }
@@ -496,7 +497,7 @@ void bind_decoder(const std::function<void*(const char*)>& at_name) {
   f_rotary = reinterpret_cast<decltype(f_rotary)>(at_name("elsa_rotary"));
   f_prefix_ws = reinterpret_cast<decltype(f_prefix_ws)>(at_name("elsa_shared_prefix_workspace_bytes"));
   f_prefix = reinterpret_cast<decltype(f_prefix)>(at_name("elsa_shared_prefix_attention"));
-  f_diff_ws = reinterpret_cast<decltype(f_diff_ws)>(at_name("elsa_differential_workspace_bytes"));
+  f_diff_ws = reinterpret_cast<decltype(f_diff_ws)>(at_name("elsa_differential_workspace_bytes_for"));
   f_diff = reinterpret_cast<decltype(f_diff)>(at_name("elsa_differential_forward"));
   f_diff_bwd_ws = reinterpret_cast<decltype(f_diff_bwd_ws)>(at_name("elsa_differential_backward_workspace_bytes"));
   f_diff_bwd = reinterpret_cast<decltype(f_diff_bwd)>(at_name("elsa_differential_backward"));

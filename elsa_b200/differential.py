@@ -79,16 +79,17 @@ def _forward(q, k, v, lam, sizes, is_causal, scale, lengths, want_state):
         lse = torch.empty((2, batch, heads, nq), device=q.device, dtype=torch.float32)
     lam, lam_ptr, lam_dtype, lam_stride = _lam_args(lam, heads, q)
     dt = _lib.dtype_code(q.dtype)
-    need = _cached_bytes("elsa_differential_workspace_bytes", dt, *sizes)
-    if need < 0:
-        raise ValueError("elsa_b200: unsupported problem size for differential_attention")
     flat = (ctypes.c_int64 * 12)(*qs, *ks, *vs, *_strides(out))
+    n = None if lengths is None else lengths.data_ptr()
     with _DeviceScope(q.device):
-        ws = torch.empty((max(need, 256),), device=q.device, dtype=torch.uint8)
+        need = int(_lib.load().elsa_differential_workspace_bytes_for(q.data_ptr(), k.data_ptr(), v.data_ptr(), n, out.data_ptr(), flat, dt, *sizes))
+        if need < 0:
+            raise ValueError("elsa_b200: unsupported problem size for differential_attention")
+        ws = torch.empty((need,), device=q.device, dtype=torch.uint8)      # (the tiles need none)
         rc = _lib.load().elsa_differential_forward(
-            q.data_ptr(), k.data_ptr(), v.data_ptr(), lam_ptr, lam_dtype, lam_stride, None if lengths is None else lengths.data_ptr(),
-            out.data_ptr(), flat, None if out2 is None else out2.data_ptr(), None if lse is None else lse.data_ptr(), ws.data_ptr(),
-            ws.numel(), dt, *sizes, int(bool(is_causal)), scale, _lib.raw_stream(q.device))
+            q.data_ptr(), k.data_ptr(), v.data_ptr(), lam_ptr, lam_dtype, lam_stride, n, out.data_ptr(), flat,
+            None if out2 is None else out2.data_ptr(), None if lse is None else lse.data_ptr(), ws.data_ptr(), need, dt, *sizes,
+            int(bool(is_causal)), scale, _lib.raw_stream(q.device))
     _lib.check(rc, "elsa_differential_forward")
     return out, out2, lse, q, k, v
 

@@ -218,3 +218,23 @@ def test_axes_that_32_bits_do_not_count_are_refused():
         with pytest.raises(ValueError, match="an axis of more than"):
             call(long(1, 2, 1, 8), long(1, 2, n, 8), long(1, 1, n, 8), 0.5)
 
+
+
+# ---- what the calls ask for ------------------------------------------------------------------------------------------
+def _differential_bytes(lib, batch, heads, kv, nq, nk, d=64, dv=128, dtype=2, q=4096, out=4096, lengths=None):
+    """Of contiguous operands (nothing is read through the addresses)."""
+    import ctypes
+    st = (ctypes.c_int64 * 12)(2 * heads * nq * d, nq * d, d, 2 * kv * nk * d, nk * d, d, kv * nk * dv, nk * dv, dv, heads * nq * dv, nq * dv, dv)
+    return lib.elsa_differential_workspace_bytes_for(q, 4096, 4096, lengths, out, st, dtype, batch, heads, kv, nq, nk, d, dv)
+
+
+def test_differential_workspace_of_a_layout(lib):
+    """What the tiles do not take goes through the split kernels, with their summaries (what they take: test_gpu_differential.py)."""
+    sizes = (2, 4, 2, 100, 300)
+    every = lib.elsa_differential_workspace_bytes(2, *sizes, 64, 128)
+    assert every > 0 and _differential_bytes(lib, *sizes, lengths=4096) == every
+    assert _differential_bytes(lib, *sizes, q=4098) == every and _differential_bytes(lib, *sizes, out=4104) == every
+    assert _differential_bytes(lib, *sizes, dtype=0) == lib.elsa_differential_workspace_bytes(0, *sizes, 64, 128)
+    assert _differential_bytes(lib, 2, 4, 2, 1, 300) == lib.elsa_differential_workspace_bytes(2, 2, 4, 2, 1, 300, 64, 128)
+    assert _differential_bytes(lib, 1, 4, 3, 100, 300) == -1 and _differential_bytes(lib, *sizes, d=136) == -1
+    assert lib.elsa_differential_workspace_bytes_for(4096, 4096, 4096, None, 4096, None, 2, *sizes, 64, 128) == -1

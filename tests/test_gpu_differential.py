@@ -460,3 +460,38 @@ def test_gradients_with_tiles_of_one_two_and_four_blocks(b, causal):
     _check_gradients(got, q, k, v, lam, dout, causal)
     assert all(torch.equal(x, y) for x, y in zip(got, _run_train(q, k, v, lam, dout, is_causal=causal)[1]))
 
+
+
+def test_tiles_ask_for_no_workspace():
+    from tests.test_decoder_cpu import _differential_bytes
+    lib = _lib.load()
+    for batch, heads, kv, n in ((2, 4, 2, 300), (2, 8, 8, 8192), (1, 16, 16, 32768), (1, 32, 8, 65536), (1, 16, 16, 131072)):
+        assert _differential_bytes(lib, batch, heads, kv, n, n) == 0
+        assert _differential_bytes(lib, batch, heads, kv, n, n, out=4104) == lib.elsa_differential_workspace_bytes(2, batch, heads, kv, n, n, 64, 128) > 0
+
+
+def _peak(call):
+    """(result, bytes that the call had allocated at its fullest, what it returned among them)"""
+    torch.cuda.synchronize()
+    torch.cuda.reset_peak_memory_stats()
+    before = torch.cuda.memory_allocated()
+    result = call()
+    torch.cuda.synchronize()
+    return result, torch.cuda.max_memory_allocated() - before
+
+
+@pytest.mark.parametrize("native", [True, False])
+def test_a_long_prompt_allocates_what_it_returns(native, monkeypatch):
+    """16 heads of 32768 tokens: the result, for a training step its state, and no scratch that grows with queries times keys."""
+    if not native:
+        monkeypatch.setattr(_lib, "host", lambda: None)
+    n, h, d, dv = 32768, 16, 64, 128
+    q, k, v = (torch.randn((1, heads, n, width), device="cuda", dtype=torch.bfloat16) for heads, width in ((2 * h, d), (2 * h, d), (h, dv)))
+    lam = torch.full((h,), 0.5, device="cuda")
+    out_bytes, state_bytes = h * n * dv * 2, 2 * h * n * 4
+    out, peak = _peak(lambda: E.differential_attention(q, k, v, lam, is_causal=True))
+    assert peak <= out_bytes + 2 ** 22
+    _check_forward(out[:, :1, -3:].contiguous(), q[:, :2, -3:], k[:, :2], v[:, :1], lam[:1], causal=True)
+    q.requires_grad_(True)
+    out2, peak = _peak(lambda: E.differential_attention_train(q, k, v, lam, is_causal=True))
+    assert torch.equal(out2, out) and peak <= 2 * out_bytes + state_bytes + 2 ** 22
