@@ -39,6 +39,34 @@ int split_width(int dtype, int64_t blocks_of_one_split, int n_keys) {
   return static_cast<int>(std::max<int64_t>(64, std::min<int64_t>(width, 1024)));
 }
 
+// Summaries grow with queries times keys: the split kernels walk a call's queries in chunks -- whole sequences, or tokens of one --
+// whose summaries fit 1 GiB, as the forward of api.cu does, through the same workspace.  A row's result is the same in any chunk.
+constexpr int64_t kSummaryBytes = 1ll << 30;
+
+struct Chunk { int seqs, tokens; };
+
+// token_bytes: the summaries of one token, all heads and parts
+Chunk chunk_of(int batch, int nq, int64_t token_bytes) {
+  const int64_t tokens = std::max<int64_t>(1, kSummaryBytes / std::max<int64_t>(1, token_bytes));
+  if (tokens >= nq) return {static_cast<int>(std::min<int64_t>(batch, tokens / nq)), nq};
+  return {1, static_cast<int>(tokens >= 32 ? tokens / 32 * 32 : tokens)};      // (whole tiles of rows)
+}
+// so few parts that one token's summaries (head_bytes of a head and part) fit
+int bounded_width(int width, int n_keys, int heads, int64_t head_bytes) {
+  const int64_t parts = std::max<int64_t>(1, kSummaryBytes / (heads * head_bytes));
+  return static_cast<int>(std::max<int64_t>(width, align_up(cdiv64(n_keys, parts), 64)));
+}
+template <typename F>
+int for_chunks(const Chunk& c, int batch, int nq, F run) {
+  for (int b = 0; b < batch; b += c.seqs)
+    for (int t = 0; t < nq; t += c.tokens) {
+      const int rc = run(b, std::min(c.seqs, batch - b), t, std::min(c.tokens, nq - t));
+      if (rc != ELSA_OK) return rc;
+    }
+  return ELSA_OK;
+}
+const void* offset(const void* p, int64_t elements, int dtype) { return p ? static_cast<const char*>(p) + elements * dtype_size(dtype) : nullptr; }
+
 // ---- attention over a shared prefix ------------------------------------------------------------------------------------
 struct PrefixPlan {
   bool tiles;                   // the prefix on the 256-row tensor-core kernel (pair_tc.cu)
@@ -100,6 +128,7 @@ int plan_prefix(int dtype, int batch, int heads, int kv_heads, int nq, int head_
 struct DiffPlan {
   bool tensor_tiles;            // the 128-row tensor-core kernels by sizes (pair_tc.cu); else the split kernels (decode.cu)
   int split_width, parts;       // of the split kernels
+  Chunk chunk;
   int64_t mz_bytes, s_bytes;
   int64_t bytes() const { return 2 * mz_bytes + s_bytes; }
 };
@@ -116,9 +145,11 @@ int plan_diff(int dtype, int batch, int heads, int kv_heads, int nq, int nk, int
   // (nq: the backward's four statistics of a head are indexed in 32 bits)
   if (rows * kv_heads > 0x1fffffff || heads > 65535 || batch > 65535 || nk > 0x3fffffff || nq > 0xfffffff) return ELSA_ERR_UNSUPPORTED;
   pl->tensor_tiles = rows_b > kSplitRows && diff_tc_sizes(dtype, head_dim, v_dim);
-  pl->split_width = nk > 0 ? split_width(dtype, static_cast<int64_t>(batch) * kv_heads * cdiv64(rows_b, dtype == ELSA_F32 ? 32 : 16), nk) : 1;
+  const int64_t head_bytes = 2 * (v_dim + 2) * 4;
+  pl->split_width = nk > 0 ? bounded_width(split_width(dtype, static_cast<int64_t>(batch) * kv_heads * cdiv64(rows_b, dtype == ELSA_F32 ? 32 : 16), nk), nk, heads, head_bytes) : 1;
   pl->parts = static_cast<int>(cdiv64(nk, pl->split_width));
-  const int64_t summaries = 2 * static_cast<int64_t>(pl->parts) * kv_heads * rows;
+  pl->chunk = chunk_of(batch, nq, static_cast<int64_t>(pl->parts) * heads * head_bytes);
+  const int64_t summaries = 2 * static_cast<int64_t>(pl->parts) * heads * pl->chunk.seqs * pl->chunk.tokens;
   pl->mz_bytes = align_up(summaries * 4, 256);
   pl->s_bytes = align_up(summaries * v_dim * 4, 256);
   return ELSA_OK;
@@ -248,21 +279,27 @@ extern "C" int elsa_differential_forward(const void* q, const void* k, const voi
     return diff_tc_fwd(d, dtype, st);
   }
   if (pl.bytes() > 0 && (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 255u) || workspace_bytes < pl.bytes())) return ELSA_ERR_WORKSPACE;
-  DecodeParams p{};
-  p.q = q; p.qs = d.qs;
-  p.batch = batch; p.heads = heads; p.kv_heads = kv_heads; p.nq = nq; p.head_dim = head_dim; p.v_dim = v_dim; p.maps = 2;
-  p.scale_log2 = d.scale_log2;
   char* ws = static_cast<char*>(workspace);
-  p.m = reinterpret_cast<float*>(ws); p.z = reinterpret_cast<float*>(ws + pl.mz_bytes); p.s = reinterpret_cast<float*>(ws + 2 * pl.mz_bytes);
-  p.lam = lam; p.lam_dtype = lam_dtype; p.lam_stride = lam_stride;
-  p.out = out; p.os = d.os; p.out2 = out2; p.lse = lse;
-  if (nk > 0) {
-    DecodeSegment& s = p.seg[p.n_segs++];
-    s.k = k; s.v = v; s.ks = d.ks; s.vs = d.vs; s.lengths = lengths; s.n_keys = nk; s.causal = is_causal;
-    s.split_width = pl.split_width; s.n_splits = pl.parts;
-  }
-  if ((rc = decode_split(p, dtype, false, st)) != ELSA_OK) return rc;
-  return decode_merge(p, pl.parts, dtype, nk > 0, st);
+  return for_chunks(pl.chunk, batch, nq, [&](int b0, int seqs, int t0, int tokens) -> int {
+    DecodeParams p{};
+    p.q = offset(q, b0 * d.qs.b + t0 * d.qs.r, dtype); p.qs = d.qs;
+    p.batch = seqs; p.heads = heads; p.kv_heads = kv_heads; p.nq = tokens; p.head_dim = head_dim; p.v_dim = v_dim; p.maps = 2;
+    p.scale_log2 = d.scale_log2;
+    p.m = reinterpret_cast<float*>(ws); p.z = reinterpret_cast<float*>(ws + pl.mz_bytes); p.s = reinterpret_cast<float*>(ws + 2 * pl.mz_bytes);
+    p.lam = lam; p.lam_dtype = lam_dtype; p.lam_stride = lam_stride;
+    const int64_t row0 = static_cast<int64_t>(b0) * heads * nq + t0;
+    p.out = const_cast<void*>(offset(out, b0 * d.os.b + t0 * d.os.r, dtype)); p.os = d.os;
+    p.out2 = const_cast<void*>(offset(out2, row0 * v_dim, dtype));
+    p.lse = lse ? lse + row0 : nullptr; p.nq_all = nq; p.map_rows = static_cast<int64_t>(batch) * heads * nq;
+    if (nk > 0) {
+      DecodeSegment& s = p.seg[p.n_segs++];
+      s.k = offset(k, b0 * d.ks.b, dtype); s.v = offset(v, b0 * d.vs.b, dtype); s.ks = d.ks; s.vs = d.vs;
+      s.lengths = lengths ? lengths + b0 : nullptr; s.n_keys = nk; s.causal = is_causal; s.tail = is_causal ? nq - t0 - tokens : 0;
+      s.split_width = pl.split_width; s.n_splits = pl.parts;
+    }
+    const int rc = decode_split(p, dtype, false, st);
+    return rc != ELSA_OK ? rc : decode_merge(p, pl.parts, dtype, nk > 0, st);
+  });
 }
 
 extern "C" int64_t elsa_differential_backward_workspace_bytes(int dtype, int batch, int heads, int kv_heads, int nq, int nk, int head_dim,

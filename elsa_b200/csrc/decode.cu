@@ -51,7 +51,7 @@ __device__ __forceinline__ bool locate(const DecodeParams& p, int tile_rows, Blo
   const int all = sg.shared ? rows_b * p.batch : rows_b;
   w.row0 = (sg.shared ? 0 : w.b * rows_b) + tile * tile_rows;
   w.n_rows = min(tile_rows, all - tile * tile_rows);
-  w.len = sg.shared || !sg.lengths ? sg.n_keys : max(0, min(sg.n_keys, sg.lengths[w.b]));
+  w.len = keys_of(sg, w.b);
   w.k0 = split * sg.split_width;
   w.k1 = min(w.len, w.k0 + sg.split_width);
   w.part = sg.first_part + split;
@@ -534,8 +534,7 @@ merge_kernel(const DecodeParams p, int n_parts) {
   for (int s = 0; s < 2; ++s)
     if (s < p.n_segs) {
       const DecodeSegment& sg = p.seg[s];
-      const int len = sg.shared || !sg.lengths ? sg.n_keys : max(0, min(sg.n_keys, sg.lengths[b]));
-      from[s] = sg.first_part + (len + sg.split_width - 1) / sg.split_width;
+      from[s] = sg.first_part + (keys_of(sg, b) + sg.split_width - 1) / sg.split_width;
       to[s] = sg.first_part + sg.n_splits;
     }
   auto written = [&](int part) { return !(part >= from[0] && part < to[0]) && !(part >= from[1] && part < to[1]); };
@@ -602,8 +601,8 @@ merge_kernel(const DecodeParams p, int n_parts) {
 #pragma unroll
       for (int e = 0; e < 4; ++e) total[e] = acc[e];
     } else {
-      const int64_t ro = (static_cast<int64_t>(b) * p.heads + h) * p.nq + t;
-      if (p.lse && lane == 0) p.lse[m * (static_cast<int64_t>(p.batch) * p.heads * p.nq) + ro] = zs != 0.f ? top + log2f(zs) : -CUDART_INF_F;
+      const int64_t ro = (static_cast<int64_t>(b) * p.heads + h) * p.nq_all + t;
+      if (p.lse && lane == 0) p.lse[m * p.map_rows + ro] = zs != 0.f ? top + log2f(zs) : -CUDART_INF_F;
       if (m == 0) {
 #pragma unroll
         for (int e = 0; e < 4; ++e) total[e] = acc[e];

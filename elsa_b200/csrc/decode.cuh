@@ -15,6 +15,7 @@ struct DecodeSegment {
   Strides ks, vs;                       // head axis of k: maps * kv heads, of v: kv heads
   const int* lengths;
   int n_keys, causal, shared;
+  int tail;                             // causal: tokens of a sequence behind the last query of this launch (0 where it has them all)
   int split_width, n_splits, first_part;
   int row_tiles;                        // set by the launcher
   int64_t blocks;                       // set by the launcher
@@ -32,11 +33,18 @@ struct DecodeParams {
   const void* lam; int lam_dtype, lam_stride;   // maps == 2: out = s1 / z1 - lam[h] s2 / z2, a value for each head or for all (lam_stride 0)
   void* out; Strides os;                // [batch, heads, nq, v_dim]
   // maps == 2, for a backward (null: not wanted): s2 / z2 as contiguous [batch, heads, nq, v_dim], log2 of each row's sum of 2^score as
-  // [map][batch * heads * nq] (-inf: no key)
+  // [map][batch * heads * nq] (-inf: no key); a launch for some of a call's rows: from its first row on, nq_all tokens of a head, map_rows
+  // rows of a map
   void* out2; float* lse;
+  int nq_all; int64_t map_rows;
 };
 
 __host__ __device__ inline int64_t decode_rows(const DecodeParams& p) { return static_cast<int64_t>(p.batch) * (p.heads / p.kv_heads) * p.nq; }
+
+// the keys of sequence b that some query of the launch may see (a tail's queries see more)
+__device__ __forceinline__ int keys_of(const DecodeSegment& s, int b) {
+  return max(0, (s.shared || !s.lengths ? s.n_keys : min(s.n_keys, s.lengths[b])) - s.tail);
+}
 
 // A kernel that was launched by launch_behind may begin while the launch before it in the stream still runs, once all of that one's blocks
 // have called let_next_begin (or ended); wait_for_previous returns when it has ended and its writes can be read.  Both do nothing in

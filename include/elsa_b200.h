@@ -379,7 +379,7 @@ int elsa_shared_prefix_attention(const void* q, const void* k_prefix, const void
  * `strides` = element strides {batch, head, row} of q, k, v, out; the elements of a row are contiguous.
  * out2, lse: NULL, or what elsa_differential_backward needs: P2 v as contiguous [batch, heads, nq, v_dim] in `dtype`, and log2 of each
  * row's sum of 2^score as [2][batch * heads * nq] fp32.  scale: positive and finite in fp32.
- * workspace (256-byte aligned): elsa_differential_workspace_bytes is enough for every layout; elsa_differential_workspace_bytes_for is what
+ * workspace (256-byte aligned, about 1 GiB at most: longer problems go through it in chunks of queries): elsa_differential_workspace_bytes is enough for every layout; elsa_differential_workspace_bytes_for is what
  * a call with these pointers and strides takes: 0 (workspace may be NULL) where it runs on the tensor-core tiles.  Nothing is read through
  * the pointers.  -1 from either for sizes that the call would refuse. */
 int64_t elsa_differential_workspace_bytes(int dtype, int batch, int heads, int kv_heads, int nq, int nk, int head_dim, int v_dim);

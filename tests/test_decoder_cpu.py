@@ -238,3 +238,15 @@ def test_differential_workspace_of_a_layout(lib):
     assert _differential_bytes(lib, 2, 4, 2, 1, 300) == lib.elsa_differential_workspace_bytes(2, 2, 4, 2, 1, 300, 64, 128)
     assert _differential_bytes(lib, 1, 4, 3, 100, 300) == -1 and _differential_bytes(lib, *sizes, d=136) == -1
     assert lib.elsa_differential_workspace_bytes_for(4096, 4096, 4096, None, 4096, None, 2, *sizes, 64, 128) == -1
+
+
+@pytest.mark.parametrize("dtype", [0, 1, 2])
+def test_differential_summaries_are_bounded(lib, dtype):
+    """The split kernels' summaries, queries times parts of the keys: no call asks for more than 1 GiB of them."""
+    size = lib.elsa_differential_workspace_bytes
+    for batch, heads, kv, nq, nk in ((2, 8, 8, 8192, 8192), (1, 16, 16, 32768, 32768), (1, 32, 8, 65536, 65536), (1, 16, 16, 131072, 131072),
+                                     (1, 128, 1, 1, 1 << 23), (1, 65535, 1, 1, 1 << 20), (4096, 32, 8, 4, 8192), (1, 1, 1, 1 << 20, 1 << 20)):
+        assert 0 < size(dtype, batch, heads, kv, nq, nk, 64, 128) <= (1 << 30) + 1024
+    # small calls: every summary at once, as before
+    parts = -(-100 // 64)
+    assert size(dtype, 2, 4, 2, 3, 100, 64, 128) == 2 * 512 + parts * 2 * 4 * 2 * 3 * 128 * 4

@@ -495,3 +495,53 @@ def test_a_long_prompt_allocates_what_it_returns(native, monkeypatch):
     q.requires_grad_(True)
     out2, peak = _peak(lambda: E.differential_attention_train(q, k, v, lam, is_causal=True))
     assert torch.equal(out2, out) and peak <= 2 * out_bytes + state_bytes + 2 ** 22
+
+
+def _rows(q, k, t0, t1):
+    """What queries t0 .. t1 of a causal call are to a call of their own: themselves and the keys up to the last one's."""
+    return q[:, :, t0:t1], k[:, :, : k.shape[2] - q.shape[2] + t1]
+
+
+@pytest.mark.parametrize("case", [(1, 2, 1, 9000, 65536, 64, 128), (9, 16, 16, 1001, 16001, 32, 64)], ids=str)
+def test_queries_in_chunks(case):
+    """Summaries of more than 1 GiB: the split kernels take tokens of a sequence, or whole sequences, in turn.  Rows on either side of the
+    chunks' borders (8064 tokens; 7 sequences), their saved P2 v and sums among them."""
+    b, h, hkv, nq, nk, d, dv = case
+    q, k, v, lam = _inputs(*case, torch.float32)
+    (out, out2, lse, *_), peak = _peak(lambda: E.differential._forward(q, k, v, lam, (b, h, hkv, nq, nk, d, dv), True, d ** -0.5, None, True))
+    assert peak <= 2 ** 30 + sum(t.numel() * 4 for t in (out, out2, lse)) + 2 ** 22
+    for i in {0, 6, 7, b - 1} & set(range(b)):
+        one = slice(i, i + 1)
+        for t0, t1 in ((0, 3), (nq // 2, nq // 2 + 2), (min(8062, nq - 4), min(8066, nq)), (nq - 3, nq)):
+            qs, ks = _rows(q[one], k[one], t0, t1)
+            vs = v[one, :, : ks.shape[2]]
+            _check_forward(out[one, :, t0:t1], qs, ks, vs, lam, causal=True)
+            for j in {0, h - 1}:
+                maps, g, _ = _maps(qs, ks, lam, True, None, None, 0, j, hkv)
+                want = maps[1].p @ vs[0, g].double()
+                limit = (maps[1].e + SUMS) * (maps[1].p @ vs[0, g].double().abs()) + 2.0 ** -24 * want.abs() * 1.01 + 2.0 ** -25
+                assert bool(((out2[i, j, t0:t1].double() - want).abs() <= limit).all())
+                # (a sum of weights is off by e and SUMS of itself, its log2 by that / ln 2; one rounding of the result, of the maximum and of the sum)
+                for m in (0, 1):
+                    off = (lse[m, i, j, t0:t1].double() - maps[m].lse2).abs()
+                    assert bool((off <= 1.5 * (maps[m].e[:, 0] + SUMS) + 3 * 2.0 ** -24 * (maps[m].lse2.abs() + 32)).all())
+
+
+@pytest.mark.parametrize("causal", [False, True])
+def test_queries_of_caches_with_lengths_in_chunks(causal):
+    """As above, bf16, behind caches of different lengths: shorter than a chunk's first query's, empty, full."""
+    b, h, hkv, nq, nk, d, dv = 4, 4, 1, 9000, 32768, 64, 128
+    q, k, v, lam = _inputs(b, h, hkv, nq, nk, d, dv, torch.bfloat16)
+    lengths = torch.tensor([0, 700, 20001, nk], dtype=torch.int32)
+    for i, n in enumerate(lengths.tolist()):
+        k[i, :, n:], v[i, :, n:] = float("nan"), float("inf")
+    got = E.differential_attention(q, k, v, lam, is_causal=causal, lengths=lengths.cuda())
+    assert not bool(got[0].any())
+    for i, n in enumerate(lengths.tolist()):
+        for t0, t1 in ((0, 2), (8062, 8066), (nq - n - 1, nq - n + 2), (nq - 3, nq)):
+            if 0 <= t0 < t1 <= nq:
+                last = n - nq + t1 if causal else n             # keys that the last of these rows sees
+                if last <= 0:
+                    assert not bool(got[i, :, t0:t1].any())
+                    continue
+                _check_forward(got[i:i + 1, :, t0:t1], q[i:i + 1, :, t0:t1], k[i:i + 1, :, :last], v[i:i + 1, :, :last], lam, causal=causal)
