@@ -71,7 +71,8 @@ const void* offset(const void* p, int64_t elements, int dtype) { return p ? stat
 struct PrefixPlan {
   bool tiles;                   // the prefix on the 256-row tensor-core kernel (pair_tc.cu)
   int prefix_width, prefix_parts, own_width, own_parts;
-  int64_t rows, mz_bytes, s_bytes;
+  Chunk chunk;
+  int64_t mz_bytes, s_bytes;
   int64_t bytes() const { return 2 * mz_bytes + s_bytes; }
 };
 
@@ -84,12 +85,12 @@ int plan_prefix(int dtype, int batch, int heads, int kv_heads, int nq, int head_
   if (head_dim > 128) return ELSA_ERR_UNSUPPORTED;
   const int64_t rows = static_cast<int64_t>(batch) * (heads / kv_heads) * nq;
   if (rows * heads > 0x3fffffff || kv_heads > 65535 || n_prefix > 0x3fffffff || n_own > 0x3fffffff) return ELSA_ERR_UNSUPPORTED;
-  pl->rows = rows;
   pl->tiles = rows > kTileRows && n_prefix >= 128 && (fold_tc_supported(dtype, head_dim, false) || fold_tcw_supported(dtype, head_dim, false));
   pl->prefix_width = pl->prefix_parts = pl->own_width = pl->own_parts = 0;
   const int tile = dtype == ELSA_F32 ? 32 : 16;          // rows of a block of the split kernels
+  const int64_t head_bytes = (head_dim + 2) * 4;         // a summary (the prefix and the own keys have half of a chunk's each)
   if (n_own > 0) {
-    pl->own_width = split_width(dtype, static_cast<int64_t>(batch) * kv_heads * cdiv64(heads / kv_heads * nq, tile), n_own);
+    pl->own_width = bounded_width(split_width(dtype, static_cast<int64_t>(batch) * kv_heads * cdiv64(heads / kv_heads * nq, tile), n_own), n_own, heads, 2 * head_bytes);
     pl->own_parts = static_cast<int>(cdiv64(n_own, pl->own_width));
   }
   if (pl->tiles) {
@@ -115,10 +116,12 @@ int plan_prefix(int dtype, int batch, int heads, int kv_heads, int nq, int head_
     }
     pl->prefix_width = static_cast<int>(best * 64);
   } else if (n_prefix > 0) {
-    pl->prefix_width = split_width(dtype, kv_heads * cdiv64(rows, tile), n_prefix);
+    pl->prefix_width = bounded_width(split_width(dtype, kv_heads * cdiv64(rows, tile), n_prefix), n_prefix, heads, 2 * head_bytes);
   }
   if (n_prefix > 0) pl->prefix_parts = static_cast<int>(cdiv64(n_prefix, pl->prefix_width));
-  const int64_t summaries = static_cast<int64_t>(pl->prefix_parts + pl->own_parts) * kv_heads * rows;
+  const int64_t parts = pl->prefix_parts + pl->own_parts;
+  pl->chunk = chunk_of(batch, nq, parts * heads * head_bytes);
+  const int64_t summaries = parts * heads * pl->chunk.seqs * pl->chunk.tokens;
   pl->mz_bytes = align_up(summaries * 4, 256);
   pl->s_bytes = align_up(summaries * head_dim * 4, 256);
   return ELSA_OK;
@@ -214,37 +217,42 @@ extern "C" int elsa_shared_prefix_attention(const void* q, const void* k_prefix,
   if (pl.bytes() > 0 && (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 255u) || workspace_bytes < pl.bytes())) return ELSA_ERR_WORKSPACE;
   auto st = static_cast<cudaStream_t>(stream);
   char* ws = static_cast<char*>(workspace);
-  DecodeParams p{};
-  p.q = q; p.qs = Strides{strides[0], strides[1], strides[2]};
-  p.batch = batch; p.heads = heads; p.kv_heads = kv_heads; p.nq = nq; p.head_dim = p.v_dim = head_dim; p.maps = 1;
-  p.scale_log2 = static_cast<float>(scale * 1.4426950408889634);
-  p.m = reinterpret_cast<float*>(ws);
-  p.z = reinterpret_cast<float*>(ws + pl.mz_bytes);
-  p.s = reinterpret_cast<float*>(ws + 2 * pl.mz_bytes);
-  p.out = out; p.os = Strides{strides[13], strides[14], strides[15]};
-  bool beside = false;                                  // the prefix's kernel has been launched
-  if (n_prefix > 0) {
-    DecodeSegment& s = p.seg[0];
-    s.k = k_prefix; s.v = v_prefix; s.ks = Strides{0, strides[3], strides[4]}; s.vs = Strides{0, strides[5], strides[6]}; s.n_keys = n_prefix; s.shared = 1;
-    s.split_width = pl.prefix_width; s.n_splits = pl.prefix_parts; s.first_part = 0;
-    // (a layout that the tensor maps do not take goes through the split kernel with the same parts)
-    if (pl.tiles && rows_tc_ok(p, dtype)) {
-      if ((rc = device_status_ok()) != ELSA_OK) return rc;
-      if ((rc = rows_tc(p, pl.prefix_width, pl.prefix_parts, dtype, st)) != ELSA_OK) return rc;
-      beside = true;
-    } else {
-      p.n_segs = 1;
+  const Strides qs{strides[0], strides[1], strides[2]}, ks{strides[7], strides[8], strides[9]}, vs{strides[10], strides[11], strides[12]};
+  const Strides os{strides[13], strides[14], strides[15]};
+  return for_chunks(pl.chunk, batch, nq, [&](int b0, int seqs, int t0, int tokens) -> int {
+    DecodeParams p{};
+    p.q = offset(q, b0 * qs.b + t0 * qs.r, dtype); p.qs = qs;
+    p.batch = seqs; p.heads = heads; p.kv_heads = kv_heads; p.nq = tokens; p.head_dim = p.v_dim = head_dim; p.maps = 1;
+    p.scale_log2 = static_cast<float>(scale * 1.4426950408889634);
+    p.m = reinterpret_cast<float*>(ws);
+    p.z = reinterpret_cast<float*>(ws + pl.mz_bytes);
+    p.s = reinterpret_cast<float*>(ws + 2 * pl.mz_bytes);
+    p.out = const_cast<void*>(offset(out, b0 * os.b + t0 * os.r, dtype)); p.os = os;
+    int rc;
+    bool beside = false;                                // the prefix's kernel has been launched
+    if (n_prefix > 0) {
+      DecodeSegment& s = p.seg[0];
+      s.k = k_prefix; s.v = v_prefix; s.ks = Strides{0, strides[3], strides[4]}; s.vs = Strides{0, strides[5], strides[6]}; s.n_keys = n_prefix; s.shared = 1;
+      s.split_width = pl.prefix_width; s.n_splits = pl.prefix_parts; s.first_part = 0;
+      // (a layout that the tensor maps do not take goes through the split kernel with the same parts)
+      if (pl.tiles && rows_tc_ok(p, dtype)) {
+        if ((rc = device_status_ok()) != ELSA_OK) return rc;
+        if ((rc = rows_tc(p, pl.prefix_width, pl.prefix_parts, dtype, st)) != ELSA_OK) return rc;
+        beside = true;
+      } else {
+        p.n_segs = 1;
+      }
     }
-  }
-  if (n_own > 0) {
-    DecodeSegment& s = p.seg[p.n_segs++];
-    s = DecodeSegment{};
-    s.k = k; s.v = v; s.ks = Strides{strides[7], strides[8], strides[9]}; s.vs = Strides{strides[10], strides[11], strides[12]};
-    s.lengths = lengths; s.n_keys = n_own; s.causal = 1;
-    s.split_width = pl.own_width; s.n_splits = pl.own_parts; s.first_part = pl.prefix_parts;
-  }
-  if ((rc = decode_split(p, dtype, beside, st)) != ELSA_OK) return rc;
-  return decode_merge(p, pl.prefix_parts + pl.own_parts, dtype, n_prefix + n_own > 0, st);
+    if (n_own > 0) {
+      DecodeSegment& s = p.seg[p.n_segs++];
+      s = DecodeSegment{};
+      s.k = offset(k, b0 * ks.b, dtype); s.v = offset(v, b0 * vs.b, dtype); s.ks = ks; s.vs = vs;
+      s.lengths = lengths ? lengths + b0 : nullptr; s.n_keys = n_own; s.causal = 1; s.tail = nq - t0 - tokens;
+      s.split_width = pl.own_width; s.n_splits = pl.own_parts; s.first_part = pl.prefix_parts;
+    }
+    if ((rc = decode_split(p, dtype, beside, st)) != ELSA_OK) return rc;
+    return decode_merge(p, pl.prefix_parts + pl.own_parts, dtype, n_prefix + n_own > 0, st);
+  });
 }
 
 extern "C" int64_t elsa_differential_workspace_bytes(int dtype, int batch, int heads, int kv_heads, int nq, int nk, int head_dim, int v_dim) {

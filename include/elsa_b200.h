@@ -363,7 +363,8 @@ int elsa_rotary(const void* q, void* q_out, const int64_t* q_strides, int q_head
  * `strides` = element strides, in this order: q {b, h, r}, k_prefix {h, r}, v_prefix {h, r}, k {b, h, r}, v {b, h, r}, out {b, h, r}; the
  * elements of a row are contiguous.  head_dim <= 128.  16-bit inputs whose rows start on 16-byte boundaries run on the tensor
  * cores.  n_prefix or n_own may be 0 (then its pointers are not looked at).  scale: positive and finite in fp32.
- * workspace (256-byte aligned): elsa_shared_prefix_workspace_bytes; -1 for sizes that the call would refuse. */
+ * workspace (256-byte aligned): elsa_shared_prefix_workspace_bytes, about 1 GiB at most (longer problems go through it in chunks of
+ * queries); -1 for sizes that the call would refuse. */
 int64_t elsa_shared_prefix_workspace_bytes(int dtype, int batch, int heads, int kv_heads, int nq, int head_dim, int n_prefix, int n_own);
 int elsa_shared_prefix_attention(const void* q, const void* k_prefix, const void* v_prefix, const void* k, const void* v, void* out,
                                  const int64_t* strides, const int* lengths, void* workspace, int64_t workspace_bytes, int dtype,

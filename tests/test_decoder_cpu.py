@@ -250,3 +250,13 @@ def test_differential_summaries_are_bounded(lib, dtype):
     # small calls: every summary at once, as before
     parts = -(-100 // 64)
     assert size(dtype, 2, 4, 2, 3, 100, 64, 128) == 2 * 512 + parts * 2 * 4 * 2 * 3 * 128 * 4
+
+
+@pytest.mark.parametrize("dtype", [0, 1, 2])
+def test_shared_prefix_summaries_are_bounded(lib, dtype):
+    size = lib.elsa_shared_prefix_workspace_bytes
+    for batch, heads, kv, nq, d, p, s in ((64, 32, 8, 4096, 128, 8192, 8192), (1, 32, 8, 32768, 128, 0, 32768), (3, 32, 8, 8000, 128, 2000, 8192),
+                                          (1, 128, 1, 1, 128, 1 << 23, 1 << 23), (4096, 32, 8, 8, 128, 100000, 4096)):
+        assert 0 < size(dtype, batch, heads, kv, nq, d, p, s) <= (1 << 30) + 1024
+    # small calls: every summary at once, as before
+    assert size(dtype, 2, 4, 2, 1, 64, 100, 50) == 2 * 256 + (2 + 1) * 2 * 2 * 2 * 64 * 4

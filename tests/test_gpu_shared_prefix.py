@@ -246,3 +246,35 @@ def test_calls_in_a_row_and_side_by_side_do_not_meet(shape):
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(beside, want))
 
+
+
+@pytest.mark.parametrize("aligned", [True, False])
+@pytest.mark.parametrize("nq,p", [(4096, 2000), (8000, 2000), (8000, 0)])
+def test_queries_in_chunks(nq, p, aligned):
+    """Summaries of more than 1 GiB (9 parts or 8 of 32 heads): tokens of a sequence, or whole sequences, in turn.  Rows on either side of
+    the chunks' borders, behind caches that are empty, shorter than a chunk's first query's, full."""
+    b, h, hkv, d, s = 4, 32, 8, 128, 8192
+    q, kp, vp, k, v = (torch.randn(shape, device="cuda", generator=torch.Generator("cuda").manual_seed(i)).half()
+                       for i, shape in enumerate(((b, h, nq, d), (hkv, p, d), (hkv, p, d), (b, hkv, s, d), (b, hkv, s, d))))
+    if not aligned:                                          # (a layout that the tile kernel does not take)
+        kp, vp = (torch.cat((t.new_zeros(1), t.flatten()))[1:].view(t.shape) for t in (kp, vp))
+    lengths = torch.tensor([0, 300, 5001, s], dtype=torch.int32)
+    for i, n in enumerate(lengths.tolist()):
+        k[i, :, n:], v[i, :, n:] = float("nan"), float("inf")
+    torch.cuda.synchronize()
+    torch.cuda.reset_peak_memory_stats()
+    before = torch.cuda.memory_allocated()
+    got = E.shared_prefix_attention(q, kp, vp, k, v, lengths=lengths.cuda())
+    assert torch.cuda.max_memory_allocated() - before <= 2 ** 30 + got.numel() * 2 + 2 ** 22
+    for i, n in enumerate(lengths.tolist()):
+        one = slice(i, i + 1)
+        # (7168 and 8064 tokens go at a time; the first own key is seen by query nq - n)
+        for t0, t1 in ((0, 2), (7166, 7170), (8062, 8066), (nq - n - 1, nq - n + 2), (nq - 3, nq)):
+            if 0 <= t0 < t1 <= nq:
+                last = n - nq + t1                           # own keys that the last of these rows sees
+                part = max(0, last)
+                rows = q[one, :, t0:t1]
+                if last <= 0:                                # none of them sees one
+                    _check(got[one, :, t0:t1], rows, kp, vp, k[one, :, :0], v[one, :, :0])
+                else:
+                    _check(got[one, :, t0:t1], rows, kp, vp, k[one, :, :part], v[one, :, :part])
