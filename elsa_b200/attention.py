@@ -180,13 +180,14 @@ def _empty_like_layout(ref: torch.Tensor, like_strides) -> torch.Tensor:
 _WS_CACHE: dict = {}
 
 
-def _cached_bytes(fn_name: str, *args) -> int:
-    """Workspace size queries are pure functions of their arguments: remember them (the per-call ctypes round trip is
-    a measurable part of a 49-token window problem)."""
-    key = (fn_name,) + args
+def _cached_bytes(fn_name: str, device: torch.device, *args) -> int:
+    """Workspace size queries are pure functions of their arguments and of the device (its number of SMs): remember them (the
+    per-call ctypes round trip is a measurable part of a 49-token window problem)."""
+    key = (fn_name, device) + args
     val = _WS_CACHE.get(key)
     if val is None:
-        val = int(getattr(_lib.load(), fn_name)(*args))
+        with _DeviceScope(device):
+            val = int(getattr(_lib.load(), fn_name)(*args))
         _WS_CACHE[key] = val
     return val
 
@@ -238,7 +239,7 @@ def _forward_impl(q, k, v, *, bias, is_causal, summary_dtype, part_width, q_chun
         row_z = torch.empty_like(row_m)
     meta = _canonical_bias(bias, batch=batch, heads=heads, seq_len=seq_len, device=q.device)
     dt, sdt = _lib.dtype_code(q.dtype), _lib.dtype_code(summary_dtype)
-    nbytes = _cached_bytes("elsa_forward_workspace_bytes", dt, sdt, batch, heads, seq_len, head_dim, int(meta.has_bias),
+    nbytes = _cached_bytes("elsa_forward_workspace_bytes", q.device, dt, sdt, batch, heads, seq_len, head_dim, int(meta.has_bias),
                            int(bool(is_causal)), part_width, q_chunk, flags)
     if nbytes < 0:
         raise ValueError("elsa_b200: unsupported problem size for the forward")

@@ -133,7 +133,7 @@ def _backward_impl(q, k, v, out, grad_out, *, bias, is_causal, row_m, row_z, wan
         dargs = (dbias.data_ptr(), meta.stride_b, meta.stride_h, meta.stride_q, meta.stride_k)
     flags |= _repeatable_flag()
     dt = _lib.dtype_code(q.dtype)
-    nbytes = _cached_bytes("elsa_backward_workspace_bytes", dt, batch, heads, seq_len, head_dim, int(meta.has_bias),
+    nbytes = _cached_bytes("elsa_backward_workspace_bytes", q.device, dt, batch, heads, seq_len, head_dim, int(meta.has_bias),
                            int(bool(is_causal)), flags)
     if nbytes < 0:
         raise ValueError("elsa_b200: unsupported problem size for the backward")
@@ -242,8 +242,8 @@ class _TwopassAttentionAutograd(torch.autograd.Function):
 
 
 # ---- packed projection output: the model hooks' path, kept short on the host ------------------------------------
-# Everything that depends only on the problem's shape (stride arrays for the C ABI, workspace sizes, dtype codes) is
-# built once per shape; a call then allocates its outputs, takes pointers and goes through ctypes.
+# Everything that depends only on the problem's shape and device (stride arrays for the C ABI, workspace sizes, dtype codes)
+# is built once per shape; a call then allocates its outputs, takes pointers and goes through ctypes.
 _PACKED_PLANS: dict = {}
 
 
@@ -260,9 +260,9 @@ class _PackedPlan:
         plain = (seq_len * self.hd, head_dim, self.hd)
         self.qkv_strides = _i64x(packed)
         self.out_strides = _i64x(plain)
-        self.fwd_ws = _cached_bytes("elsa_forward_workspace_bytes", self.dt, _lib.dtype_code(summary_dtype), batch, heads,
+        self.fwd_ws = _cached_bytes("elsa_forward_workspace_bytes", qkv.device, self.dt, _lib.dtype_code(summary_dtype), batch, heads,
                                     seq_len, head_dim, int(has_bias), int(is_causal), part_width, q_chunk, 0)
-        self.bwd_ws = _cached_bytes("elsa_backward_workspace_bytes", self.dt, batch, heads, seq_len, head_dim,
+        self.bwd_ws = _cached_bytes("elsa_backward_workspace_bytes", qkv.device, self.dt, batch, heads, seq_len, head_dim,
                                     int(has_bias), int(is_causal), 0)
         self.bwd_strides = {}                    # keyed by grad_out's strides: q, k, v, out, dout, dq, dk, dv
 
@@ -276,7 +276,7 @@ class _PackedPlan:
 
 
 def _packed_plan(qkv, has_bias, is_causal, summary_dtype, part_width, q_chunk):
-    key = (tuple(qkv.shape), qkv.dtype, has_bias, is_causal, summary_dtype, part_width, q_chunk)
+    key = (tuple(qkv.shape), qkv.dtype, qkv.device, has_bias, is_causal, summary_dtype, part_width, q_chunk)
     plan = _PACKED_PLANS.get(key)
     if plan is None:
         plan = _PACKED_PLANS[key] = _PackedPlan(qkv, has_bias, is_causal, summary_dtype, part_width, q_chunk)

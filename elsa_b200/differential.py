@@ -162,7 +162,7 @@ class _DifferentialAutograd(torch.autograd.Function):
             keep = keep.contiguous()
             lam_ptr, lam_stride = keep.data_ptr(), 1
         dt = _lib.dtype_code(q.dtype)
-        need = _cached_bytes("elsa_differential_backward_workspace_bytes", dt, *ctx.sizes)
+        need = _cached_bytes("elsa_differential_backward_workspace_bytes", q.device, dt, *ctx.sizes)
         flat = (ctypes.c_int64 * 24)(*_strides(q), *_strides(k), *_strides(v), *_strides(out), *gs, *_strides(dq), *_strides(dk), *_strides(dv))
         with _DeviceScope(q.device):
             ws = torch.empty((max(need, 256),), device=q.device, dtype=torch.uint8)

@@ -104,7 +104,7 @@ def shared_prefix_attention(
     (k_prefix, kps), (v_prefix, vps), (k, ks), (v, vs) = (_readable(t) for t in (k_prefix, v_prefix, k, v))
     out = _empty_like_layout(q, q.stride())
     dt = _lib.dtype_code(q.dtype)
-    need = _cached_bytes("elsa_shared_prefix_workspace_bytes", dt, batch, heads, kv_heads, nq, dim, n_prefix, n_own)
+    need = _cached_bytes("elsa_shared_prefix_workspace_bytes", q.device, dt, batch, heads, kv_heads, nq, dim, n_prefix, n_own)
     if need < 0:
         raise ValueError("elsa_b200: unsupported problem size for shared_prefix_attention")
     flat = (ctypes.c_int64 * 16)(*qs, *kps, *vps, *ks, *vs, *_strides(out))

@@ -178,3 +178,30 @@ def test_the_c_library_needs_no_torch_and_comes_first(lib, monkeypatch):
             f"runpy.run_path({build.__file__!r}, run_name='__main__')")
     res = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=600)
     assert res.returncode == 0 and res.stdout.strip() == build.LIB_PATH, res.stderr
+
+
+def test_workspace_sizes_are_asked_for_and_kept_for_each_device(monkeypatch):
+    """They depend on the number of SMs: of two different GPUs each gets its own, asked for while it is the current one."""
+    import contextlib
+    from elsa_b200 import _lib, attention
+    current, asked = [0], []
+
+    @contextlib.contextmanager
+    def scope(device):
+        before, current[0] = current[0], device.index
+        yield
+        current[0] = before
+
+    class Library:
+        @staticmethod
+        def elsa_size(n):
+            asked.append(current[0])
+            return n * (100 + current[0])
+
+    monkeypatch.setattr(attention, "_DeviceScope", scope)
+    monkeypatch.setattr(attention, "_WS_CACHE", {})
+    monkeypatch.setattr(_lib, "load", lambda: Library)
+    devices = [torch.device("cuda", i) for i in (0, 1)]
+    for _ in range(2):
+        assert [attention._cached_bytes("elsa_size", d, 7) for d in devices] == [700, 707]
+    assert asked == [0, 1]
