@@ -435,13 +435,6 @@ def twopass_attention_qkvpacked(qkv: torch.Tensor, *, bias: Optional[torch.Tenso
     k, v are read in place after it as well)."""
     if qkv.dim() != 5 or qkv.shape[2] != 3:
         raise ValueError("qkv must have shape [B,N,3,H,D]")
-    if rotary is not None:
-        from .attention import twopass_attention
-        q, k, v = qkv.permute(2, 0, 3, 1, 4).unbind(0)
-        q, k = rotary.apply(q, k)
-        if not train:
-            fwd_kwargs = {name: val for name, val in fwd_kwargs.items() if not name.startswith("bwd_")}
-        return (twopass_attention_train if train else twopass_attention)(q, k, v, bias=bias, is_causal=is_causal, **fwd_kwargs)
     # the backward tile hints of twopass_attention_train are validated and advisory, as there
     if fwd_kwargs.get("bwd_input_precision", "auto") not in ("auto", "ieee", "tf32", "tf32x3"):
         raise ValueError("input_precision must be 'auto', 'ieee', 'tf32', or 'tf32x3'")
@@ -449,6 +442,11 @@ def twopass_attention_qkvpacked(qkv: torch.Tensor, *, bias: Optional[torch.Tenso
         _validate_warps("num_warps", fwd_kwargs["bwd_num_warps"])
     if fwd_kwargs:
         fwd_kwargs = {name: val for name, val in fwd_kwargs.items() if not name.startswith("bwd_")}
+    if rotary is not None:
+        from .attention import twopass_attention
+        q, k, v = qkv.permute(2, 0, 3, 1, 4).unbind(0)
+        q, k = rotary.apply(q, k)
+        return (twopass_attention_train if train else twopass_attention)(q, k, v, bias=bias, is_causal=is_causal, **fwd_kwargs)
     if qkv.is_cuda and not fwd_kwargs.get("reference_rounding", False):
         host, keywords = _lib.host(), _native_keywords(fwd_kwargs)
         if host is not None and keywords is not None:

@@ -260,3 +260,17 @@ def test_shared_prefix_summaries_are_bounded(lib, dtype):
         assert 0 < size(dtype, batch, heads, kv, nq, d, p, s) <= (1 << 30) + 1024
     # small calls: every summary at once, as before
     assert size(dtype, 2, 4, 2, 1, 64, 100, 50) == 2 * 256 + (2 + 1) * 2 * 2 * 2 * 64 * 4
+
+
+@pytest.mark.parametrize("train", [True, False])
+@pytest.mark.parametrize("rotary", [True, False])
+def test_packed_attention_checks_backward_hints_with_and_without_rotary(rotary, train):
+    from elsa_b200.attention_bwd import twopass_attention_qkvpacked
+    qkv = torch.zeros(1, 4, 3, 2, 16)
+    kw = {"rotary": E.Rotary(E.rotary_frequencies(16)[0])} if rotary else {}
+    with pytest.raises(ValueError, match="input_precision"):
+        twopass_attention_qkvpacked(qkv, train=train, bwd_input_precision="fp4", **kw)
+    with pytest.raises(ValueError, match="num_warps"):
+        twopass_attention_qkvpacked(qkv, train=train, bwd_num_warps=3, **kw)
+    with pytest.raises(ValueError, match="CUDA"):
+        twopass_attention_qkvpacked(qkv, train=train, bwd_input_precision="tf32", bwd_num_warps=4, bwd_block_m=64, **kw)
