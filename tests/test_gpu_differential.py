@@ -545,3 +545,57 @@ def test_queries_of_caches_with_lengths_in_chunks(causal):
                     assert not bool(got[i, :, t0:t1].any())
                     continue
                 _check_forward(got[i:i + 1, :, t0:t1], q[i:i + 1, :, t0:t1], k[i:i + 1, :, :last], v[i:i + 1, :, :last], lam, causal=causal)
+
+
+def _planned_parts(dtype, b, h, hkv, nq, nk, d, dv):
+    """Parts of the keys that the split kernels take (from the bytes of their summaries; calls of one chunk)."""
+    every = _lib.load().elsa_differential_workspace_bytes({torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}[dtype], b, h, hkv, nq, nk, d, dv)
+    return every // (2 * b * h * nq * (dv + 2) * 4)          # (padding: less than a part's)
+
+
+@pytest.mark.parametrize("growing", [False, True])
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("case", [(64, 8, 8, 1, 2000, 64, 128), (64, 32, 8, 3, 1500, 64, 128), (70, 8, 8, 2, 1025, 32, 64), (48, 16, 8, 9, 1300, 48, 96)], ids=str)
+def test_many_keys_of_one_split(case, dtype, growing):
+    """Enough caches that a split has about a thousand keys: a warp's ring of stages goes round many times, its sources move on, and sums
+    gather over its chunks -- up to 8 rows of a key head and more, caches that end anywhere in a split.  Growing keys: the maximum
+    moves again and again after there are sums."""
+    b, h, hkv, nq, nk, d, dv = case
+    q, k, v, lam = _inputs(*case, dtype, scale=2.0 if growing else 1.0)
+    if growing:
+        k = (k.float() * torch.linspace(0.05, 2.0, nk, device="cuda")[:, None]).to(dtype)
+    parts = _planned_parts(dtype, *case)
+    assert parts == -(-nk // 1024)                           # 16 chunks of 16 keys for each warp
+    lengths = torch.randint(0, nk + 1, (b,), generator=torch.Generator().manual_seed(4), dtype=torch.int32)
+    lengths[:6] = torch.tensor([nk, nk - 1, 1024, 1023, 65, 0])
+    for i, n in enumerate(lengths.tolist()):
+        k[i, :, n:], v[i, :, n:] = float("nan"), float("inf")
+    got = E.differential_attention(q, k, v, lam, is_causal=True, lengths=lengths.cuda())
+    for rows in (slice(0, 8), slice(b - 3, b)):
+        # (what stands behind the last key: NaN would reach the definition's products)
+        _check_forward(got[rows], q[rows], torch.nan_to_num(k[rows]), torch.nan_to_num(v[rows], posinf=0.0), lam, causal=True, lengths=lengths[rows])
+    assert torch.equal(got, E.differential_attention(q, k, v, lam, is_causal=True, lengths=lengths.cuda()))
+
+
+@pytest.mark.parametrize("causal", [False, True])
+def test_many_keys_of_one_split_fp32(causal):
+    """As above for the kernel of any type: a block's 32-key tiles, the running maximum, sums over them."""
+    case = (40, 8, 8, 5, 2100, 64, 128)
+    q, k, v, lam = _inputs(*case, torch.float32, scale=2.0)
+    k *= torch.linspace(0.05, 2.0, 2100, device="cuda")[:, None]
+    assert _planned_parts(torch.float32, *case) <= 6         # at least ten tiles each
+    _check_forward(E.differential_attention(q, k, v, lam, is_causal=causal)[-4:], q[-4:], k[-4:], v[-4:], lam, causal=causal)
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("causal", [False, True])
+def test_growing_scores_over_many_tiles(causal, dtype):
+    """The tile kernel, 33 key tiles: the maximum moves again and again after O holds sums."""
+    case = (1, 2, 1, 150, 2083, 64, 128)
+    q, k, v, lam = _inputs(*case, dtype, scale=2.0)
+    k = (k.float() * torch.linspace(0.05, 2.0, 2083, device="cuda")[:, None]).to(dtype)
+    _check_forward(E.differential_attention(q, k, v, lam, is_causal=causal), q, k, v, lam, causal=causal)
+    q = q * 0.25                                             # (gradients: weights of more than one key)
+    dout = _normal((1, 2, 150, 128), dtype, 21)
+    out, got = _run_train(q, k, v, lam, dout, is_causal=causal)
+    _check_gradients(got, q, k, v, lam, dout, causal)

@@ -278,3 +278,47 @@ def test_queries_in_chunks(nq, p, aligned):
                     _check(got[one, :, t0:t1], rows, kp, vp, k[one, :, :0], v[one, :, :0])
                 else:
                     _check(got[one, :, t0:t1], rows, kp, vp, k[one, :, :part], v[one, :, :part])
+
+
+def _planned_parts(dtype, b, h, hkv, nq, d, p, s):
+    """(parts of the prefix, parts of the own caches), from the bytes of their summaries (calls of one chunk)."""
+    size = _lib.load().elsa_shared_prefix_workspace_bytes
+    code, row = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}[dtype], b * h * nq * (d + 2) * 4
+    own = size(code, b, h, hkv, nq, d, 0, s) // row if s else 0
+    return size(code, b, h, hkv, nq, d, p, s) // row - own, own
+
+
+@pytest.mark.parametrize("aligned", [True, False])
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("case", [(256, 32, 8, 1, 128, 6001, 1100), (256, 32, 8, 1, 64, 6001, 1100), (200, 16, 8, 3, 96, 5000, 1025), (300, 8, 8, 2, 40, 7777, 40)], ids=str)
+def test_many_tiles_of_one_part(case, dtype, aligned):
+    """Enough rows that a part of the prefix has twenty or more 64-key tiles: the ring of stages goes round, both P buffers are used again,
+    and the maximum of growing keys moves after O holds sums; beside it caches with about a thousand keys in a split.  Not aligned: the
+    same wide parts on the split kernel."""
+    b, h, hkv, nq, d, p, s = case
+    q, kp, vp, k, v = _inputs(b, h, hkv, nq, d, p, s, dtype, scale=1.5)
+    kp = (kp.float() * torch.linspace(0.05, 1.6, p, device="cuda")[:, None]).to(dtype)
+    k = (k.float() * torch.linspace(0.5, 2.0, s, device="cuda")[:, None]).to(dtype)
+    if not aligned:
+        kp, vp = (torch.cat((t.new_zeros(1), t.flatten()))[1:].view(t.shape) for t in (kp, vp))
+    prefix_parts, own_parts = _planned_parts(dtype, *case)
+    assert p / prefix_parts >= 20 * 64 and own_parts == -(-s // 1024)
+    lengths = torch.randint(0, s + 1, (b,), generator=torch.Generator().manual_seed(4), dtype=torch.int32)
+    lengths[:5] = torch.tensor([s, s - 1, min(s, 1024), 17, 0])
+    for i, n in enumerate(lengths.tolist()):
+        k[i, :, n:], v[i, :, n:] = float("nan"), float("inf")
+    got = E.shared_prefix_attention(q, kp, vp, k, v, lengths=lengths.cuda())
+    for rows in (slice(0, 6), slice(62, 66), slice(b - 3, b)):
+        _check(got[rows], q[rows], kp, vp, k[rows], v[rows], lengths=lengths[rows])
+    assert torch.equal(got, E.shared_prefix_attention(q, kp, vp, k, v, lengths=lengths.cuda()))
+
+
+def test_many_tiles_of_one_split_fp32():
+    case = (200, 8, 8, 1, 64, 3001, 1100)
+    q, kp, vp, k, v = _inputs(*case, torch.float32, scale=1.5)
+    kp *= torch.linspace(0.05, 1.6, 3001, device="cuda")[:, None]
+    prefix_parts, own_parts = _planned_parts(torch.float32, *case)
+    assert 3001 / prefix_parts >= 128 and own_parts <= 2
+    got = E.shared_prefix_attention(q, kp, vp, k, v)
+    for rows in (slice(0, 4), slice(197, 200)):
+        _check(got[rows], q[rows], kp, vp, k[rows], v[rows])
