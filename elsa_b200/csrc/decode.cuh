@@ -9,7 +9,7 @@ namespace elsa {
 
 // One key cache.  shared: [kv heads, n_keys, .] for all sequences (batch strides unused), every query sees every key.
 // Otherwise [batch, kv heads, n_keys, .]: sequence b has lengths[b] keys (null: n_keys) and, where causal, its query i of nq
-// sees the first lengths[b] - nq + i + 1 of them.  Keys from lengths[b] on are never read.
+// sees the first lengths[b] - tail - nq + i + 1 of them.  Keys from lengths[b] on are never read.
 struct DecodeSegment {
   const void* k; const void* v;
   Strides ks, vs;                       // head axis of k: maps * kv heads, of v: kv heads

@@ -111,7 +111,10 @@ def differential_attention(
     one for each output head (`differential_lambda`).  is_causal: the queries are the last Nq tokens, query i sees the first
     Nk - Nq + i + 1 keys.  lengths: int32 [B] on the device: sequence b has lengths[b] keys instead of Nk (a cache with room to grow;
     nothing behind them is read).  A query without any key gives zeros.  D, Dv <= 128; fp16, bf16 or fp32; rows of contiguous
-    elements are read in place.  scale: 1 / sqrt(D) by default.  Forward only: see `differential_attention_train`.
+    elements are read in place.  16-bit inputs run on the tensor cores' 16-bit instructions with D <= 64, D and Dv multiples of 8 and
+    rows on 16-byte boundaries; all others, and fp32, on fp32 arithmetic that is several times slower.  Of the former, calls without
+    `lengths` and with more than 64 rows for a key head need no scratch memory, all others at most 1 GiB.  scale: 1 / sqrt(D) by default.
+    Forward only: the result has no gradients, whatever the inputs ask for; see `differential_attention_train`.
     Returns [B, H, Nq, Dv]."""
     if isinstance(q, torch.Tensor) and q.is_cuda:
         host = _lib.host()
@@ -185,7 +188,7 @@ def differential_attention_train(
 ) -> torch.Tensor:
     """Differentiable `differential_attention` (without lengths), in q, k, v and, where it is a tensor, lam: the forward keeps P2 v and each
     row's log sum, the backward recomputes the maps.  Gradients repeat bit for bit; those of shared key heads and of a shared lam are
-    summed."""
+    summed.  Rows that the tensor cores' 16-bit instructions would take but for their addresses or strides are copied first."""
     if isinstance(q, torch.Tensor) and q.is_cuda:
         host = _lib.host()
         if host is not None:

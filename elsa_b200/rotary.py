@@ -303,7 +303,9 @@ def rotary_embedding(
 
 class Rotary(NamedTuple):
     """Rotary positions as one value, for calls that apply them on the way: `twopass_attention_qkvpacked(..., rotary=Rotary(...))` and the
-    ViT hooks (`patch_timm_attention(model, elsa_kwargs={"rotary": Rotary(...)})`).  The fields are `rotary_embedding`'s arguments."""
+    ViT hooks (`patch_timm_attention(model, elsa_kwargs={"rotary": Rotary(...)})`).  The fields are `rotary_embedding`'s arguments; its
+    tensors are no part of a model and do not move with it (frequencies would lose their 64 bits to `model.half()`): make them on the
+    device that the model runs on."""
 
     frequencies: torch.Tensor
     positions: Optional[torch.Tensor] = None

@@ -63,7 +63,8 @@ def shared_prefix_attention(
     behind them is read.  The queries are the last Nq of those tokens: query i sees the prefix and the first
     lengths[b] - Nq + i + 1 own keys (the prefix alone where that is not positive).  H is a multiple of Hkv; consecutive query
     heads share a key head.  P or S may be 0; a query without any key gives zeros.  D <= 128; fp16, bf16 or fp32; rows of D
-    contiguous elements are read in place, whatever the other strides.  scale: 1 / sqrt(D) by default.  Forward only.
+    contiguous elements are read in place, whatever the other strides.  scale: 1 / sqrt(D) by default.  Forward only: the result has no
+    gradients, whatever the inputs ask for.  Scratch memory: the summaries of a chunk of the queries, 1 GiB at most.
     Returns [B, H, Nq, D]."""
     if isinstance(q, torch.Tensor) and q.is_cuda:
         host = _lib.host()
