@@ -40,7 +40,9 @@ int split_width(int dtype, int64_t blocks_of_one_split, int n_keys) {
 }
 
 // Summaries grow with queries times keys: the split kernels walk a call's queries in chunks -- whole sequences, or tokens of one --
-// whose summaries fit 1 GiB, as the forward of api.cu does, through the same workspace.  A row's result is the same in any chunk.
+// whose summaries fit 1 GiB, as the forward of api.cu does, through the same workspace.  A row's result is the same in any chunk (but
+// in one of at most 8 rows of a key head, whose weights the 16-bit split kernel holds to twice the bits).  Measured, fp32, causal,
+// (1, 16 heads, 16384 tokens, 64 / 128): 41.2 ms in five chunks, 41.4 with all summaries, 4 GiB, at once.
 constexpr int64_t kSummaryBytes = 1ll << 30;
 
 struct Chunk { int seqs, tokens; };
